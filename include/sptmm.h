@@ -50,7 +50,8 @@ typedef enum sptmm_format {
     SPTMM_FMT_I2S = 5
 } sptmm_format;
 
-typedef enum sptmm_dtype { SPTMM_I8 = 0, SPTMM_F16 = 1, SPTMM_F32 = 2 } sptmm_dtype;
+/* SPTMM_BF16: the attention operators only; the matmuls take the first three */
+typedef enum sptmm_dtype { SPTMM_I8 = 0, SPTMM_F16 = 1, SPTMM_F32 = 2, SPTMM_BF16 = 3 } sptmm_dtype;
 
 /* bit flags for the `flags` argument of the launch functions */
 enum {
@@ -465,6 +466,105 @@ int sptmm_splitk_output(const sptmm_splitk *s, void **C, uint32_t *width);
 int sptmm_splitk_status(sptmm_splitk *s, uint32_t *status);
 int sptmm_splitk_set_wait_limit(sptmm_splitk *s, uint64_t polls);
 int sptmm_splitk_free(sptmm_splitk *s);
+
+/* ---- attention: what stands between the qkv product and the o product of a layer ----------------- */
+
+/* No counterpart in the reference, whose only operator is the matmul (main.cu:993-1961).  Three calls:
+ *   sptmm_rotate_heads      the fused qkv rows -> normalised, rotated 16-bit heads, stored where
+ *                           attention reads them: packed rows and / or the slots of a paged cache
+ *   sptmm_attention_prompt  whole prompts over packed keys and values
+ *   sptmm_attention_decode  one new token per sequence over a paged cache, optionally behind a prefix
+ *                           that the whole batch shares
+ * Common rules
+ *  - `dtype` is SPTMM_F16 or SPTMM_BF16, the type of Q, K, V, O and the cache.  Scores, softmax
+ *    statistics, norms and sums are fp32; a softmax weight is rounded to `dtype` before it multiplies
+ *    a value, an output once at the end.
+ *  - `heads` query heads share `kv_heads` key and value heads: head h reads key head
+ *    h / (heads / kv_heads); heads is a multiple of kv_heads, at most 128 times it.
+ *  - head_dim is a multiple of 8 up to 128.  A row of Q holds its heads back to back (head h at
+ *    h * head_dim); ld* is the number of elements between rows (0 = back to back), a multiple of 8,
+ *    so that Q, K and V may be column ranges of one fused row.  Device addresses are 16-byte aligned;
+ *    outputs overlap no input.
+ *  - Lengths, offsets, positions, slots and page numbers are device int32: nothing of the batch's
+ *    composition is read by the host, so a captured graph may be replayed with other contents.
+ *    What they name beyond a buffer's end (a slot or page outside the cache, an offset outside its
+ *    rows) is left out, not followed.
+ *  - A query without any visible key gives a row of zeros.
+ *  - No call allocates or synchronises.  SPTMM_LAUNCH_PDL in `flags` as for the matmuls. */
+
+/* A paged cache.  Element (page p, key head h, slot s, channel d) of k or v lies at
+ *     p * page_stride + (h * page_size + s) * head_dim + d.
+ * page_size: 16, 32, 64 or 128 tokens.  page_stride (elements, a multiple of 8): 0 = pages back to
+ * back, kv_heads * page_size * head_dim; larger where k and v, or several layers, share a page. */
+typedef struct sptmm_kv_cache {
+    void *k, *v;
+    uint32_t dtype, n_pages, page_size, kv_heads, head_dim;
+    uint32_t reserved;               /* 0 */
+    uint64_t page_stride;
+} sptmm_kv_cache;
+
+/* Every token's fused row q heads | k heads | v heads is read once.  For each query and key head x:
+ *     x *= w / sqrt(mean(x^2) + eps)             w = q_norm or k_norm (device float[head_dim]); NULL: no norm
+ *     (a, b) -> (a cos t - b sin t, a sin t + b cos t),   t = positions[token] * inv_freq[i]
+ * for the rot_dim / 2 channel pairs of the first rot_dim channels: pair i is channels (i, i + rot_dim/2),
+ * or (2i, 2i+1) when `interleaved`.  Values are rounded only.  The angle is formed in 64 bits, so far
+ * positions lose nothing.
+ *  - inv_freq: HOST array of rot_dim / 2 doubles, copied by the call.  rot_dim: a multiple of 8, at most
+ *    head_dim; 0 = no rotation (inv_freq and positions may be NULL).
+ *  - in_dtype: F32 (what sptmm_gemv_scaled leaves), F16 or BF16; ldqkv a multiple of 4 elements (F32) or 8.
+ *  - Q: T x heads; K and V: T x kv_heads packed rows, both or neither; cache with slots: token t's key and
+ *    value go to slot slots[t] % page_size of page slots[t] / page_size; a negative slot, or one past the
+ *    cache, is not stored.  No two tokens of a call may name the same slot (which one's channels stay is
+ *    then undefined).  K / V or the cache or both must be given. */
+typedef struct sptmm_rotate_params {
+    const void *QKV;
+    const float *q_norm, *k_norm;
+    const double *inv_freq;
+    const int32_t *positions, *slots;
+    void *Q, *K, *V;
+    const sptmm_kv_cache *cache;
+    uint64_t ldqkv, ldq, ldk, ldv;
+    uint32_t T, heads, kv_heads, head_dim, in_dtype, dtype, rot_dim, interleaved;
+    float eps;
+} sptmm_rotate_params;
+int sptmm_rotate_heads(const sptmm_rotate_params *p, uint32_t flags, void *stream);
+
+/* Attention over packed sequences: sequence s owns rows q_offsets[s] .. q_offsets[s+1] of Q and O and rows
+ * k_offsets[s] .. k_offsets[s+1] of K and V (n_seqs + 1 non-decreasing offsets each; k_offsets may be
+ * q_offsets).  Query i of n, over m keys, sees keys 0 .. i + m - n when `causal` (the last query sees the
+ * last key; queries before the first key see none), all m otherwise.
+ *     O = softmax(scale * Q K^T) V        scale 0 = 1 / sqrt(head_dim)
+ * T and Tk: rows of Q / O and of K / V.  Rows of O that belong to no sequence are left as they were. */
+typedef struct sptmm_prompt_params {
+    const void *Q, *K, *V;
+    void *O;
+    const int32_t *q_offsets, *k_offsets;
+    uint64_t ldq, ldk, ldv, ldo;
+    uint32_t n_seqs, T, Tk, heads, kv_heads, head_dim, dtype, causal;
+    float scale;
+} sptmm_prompt_params;
+int sptmm_attention_prompt(const sptmm_prompt_params *p, uint32_t flags, void *stream);
+
+/* One query row per sequence: softmax over the first prefix_len keys of the pages in prefix_table (the
+ * same for every sequence, read once for all of them) and then the first lengths[b] keys of the pages in
+ * row b of `table` (B x max_pages).  lengths[b] counts the new token if its key is in the cache already;
+ * it is cut to 0 .. max_pages * page_size.  prefix_table: ceil(prefix_len / page_size) pages.
+ * workspace: device memory of sptmm_attention_decode_workspace() bytes (16-byte aligned, contents
+ * irrelevant) for the parts of a split sequence; calls that may run at the same time, or graphs replayed
+ * at the same time, need one each.  cache: host struct, read during the call only. */
+typedef struct sptmm_decode_params {
+    const void *Q;
+    void *O;
+    const sptmm_kv_cache *cache;
+    const int32_t *lengths, *table, *prefix_table;
+    void *workspace;
+    uint64_t workspace_bytes, ldq, ldo;
+    uint32_t B, heads, max_pages, prefix_len;
+    float scale;
+} sptmm_decode_params;
+/* 0 on bad arguments.  Grows with B * heads, not with the sequences' lengths. */
+uint64_t sptmm_attention_decode_workspace(uint32_t B, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t prefix_len);
+int sptmm_attention_decode(const sptmm_decode_params *p, uint32_t flags, void *stream);
 
 /* ---- small device helpers so a C caller needs no CUDA headers ------------------------------ */
 int sptmm_device_count(int *count);

@@ -23,7 +23,7 @@ TUNING = os.environ.get("SPTMM_B200_TUNING", "") not in ("", "0")
 LIB_PATH = os.path.join(_PKG, "libsptmm_tuning.so" if TUNING else "libsptmm.so")
 
 FMT_U16_DIV, FMT_DELTA_DIV256, FMT_U16_V256, FMT_DELTA_LANE, FMT_I2S = 1, 2, 3, 4, 5
-I8, F16, F32 = 0, 1, 2
+I8, F16, F32, BF16 = 0, 1, 2, 3          # BF16: the attention operators only
 X_COLMAJOR, C_COLMAJOR, LAUNCH_PDL = 1, 2, 4
 
 _NP_DTYPE = {I8: np.int8, F16: np.float16, F32: np.float32}
@@ -114,6 +114,10 @@ def _load() -> C.CDLL:
         "sptmm_splitk_status": (i32, [vp, C.POINTER(u32)]),
         "sptmm_splitk_set_wait_limit": (i32, [vp, u64]),
         "sptmm_splitk_free": (i32, [vp]),
+        "sptmm_rotate_heads": (i32, [vp, u32, vp]),
+        "sptmm_attention_prompt": (i32, [vp, u32, vp]),
+        "sptmm_attention_decode_workspace": (u64, [u32, u32, u32, u32, u32]),
+        "sptmm_attention_decode": (i32, [vp, u32, vp]),
         "sptmm_device_count": (i32, [C.POINTER(C.c_int)]),
         "sptmm_set_device": (i32, [C.c_int]),
         "sptmm_dev_alloc": (i32, [C.POINTER(vp), u64]),
@@ -145,6 +149,7 @@ EXPORTS = ["sptmm_last_error", "sptmm_version", "sptmm_gen_ternary_fixed", "sptm
            "sptmm_splitk_k_range", "sptmm_splitk_col_range", "sptmm_splitk_arena_bytes", "sptmm_splitk_create", "sptmm_splitk_forward",
            "sptmm_splitk_clear", "sptmm_splitk_barrier", "sptmm_splitk_accumulate", "sptmm_splitk_output", "sptmm_splitk_status",
            "sptmm_splitk_set_wait_limit", "sptmm_splitk_free",
+           "sptmm_rotate_heads", "sptmm_attention_prompt", "sptmm_attention_decode_workspace", "sptmm_attention_decode",
            "sptmm_device_count", "sptmm_set_device", "sptmm_dev_alloc", "sptmm_dev_free",
            "sptmm_memcpy_h2d", "sptmm_memcpy_d2h", "sptmm_device_sync", "sptmm_stream_wait"]
 
@@ -444,6 +449,84 @@ def quantize_absmax(X, M: int, K: int, out, scale=None, ldx: int = 0, shard: int
     """int32 rows -> int8 with a per-row absmax scale (sptmm_quantize_absmax); device buffers."""
     check(lib.sptmm_quantize_absmax(_ptr(X), M, K, ldx, shard, 1 if pair else 0, _ptr(out),
                                     _ptr(scale) if scale is not None else None, flags, stream))
+
+
+class _KVCacheStruct(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_uint32), ("n_pages", C.c_uint32), ("page_size", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("reserved", C.c_uint32), ("page_stride", C.c_uint64)]
+
+
+class _RotateParams(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("QKV", "q_norm", "k_norm", "inv_freq", "positions", "slots", "Q", "K", "V", "cache")]
+                + [(n, C.c_uint64) for n in ("ldqkv", "ldq", "ldk", "ldv")]
+                + [(n, C.c_uint32) for n in ("T", "heads", "kv_heads", "head_dim", "in_dtype", "dtype", "rot_dim", "interleaved")]
+                + [("eps", C.c_float)])
+
+
+class _PromptParams(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("Q", "K", "V", "O", "q_offsets", "k_offsets")]
+                + [(n, C.c_uint64) for n in ("ldq", "ldk", "ldv", "ldo")]
+                + [(n, C.c_uint32) for n in ("n_seqs", "T", "Tk", "heads", "kv_heads", "head_dim", "dtype", "causal")]
+                + [("scale", C.c_float)])
+
+
+class _DecodeParams(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("Q", "O", "cache", "lengths", "table", "prefix_table", "workspace")]
+                + [(n, C.c_uint64) for n in ("workspace_bytes", "ldq", "ldo")]
+                + [(n, C.c_uint32) for n in ("B", "heads", "max_pages", "prefix_len")] + [("scale", C.c_float)])
+
+
+def _opt(x):
+    return _ptr(x) if x is not None else None
+
+
+class KVCache:
+    """A paged key/value cache in memory the caller owns (sptmm_kv_cache): element (page, head, slot,
+    channel) of k and v at page * page_stride + (head * page_size + slot) * head_dim + channel."""
+
+    def __init__(self, k, v, n_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: int = F16, page_stride: int = 0):
+        self._keep = (k, v)
+        self.struct = _KVCacheStruct(_ptr(k), _ptr(v), dtype, n_pages, page_size, kv_heads, head_dim, 0, page_stride)
+
+
+def rotate_heads(QKV, T: int, heads: int, kv_heads: int, head_dim: int, positions, inv_freq, Q, in_dtype: int = F32, dtype: int = F16,
+                 q_norm=None, k_norm=None, eps: float = 1e-6, interleaved: bool = False, K=None, V=None,
+                 cache: Optional[KVCache] = None, slots=None, ldqkv: int = 0, ldq: int = 0, ldk: int = 0, ldv: int = 0,
+                 flags: int = 0, stream: int = 0) -> None:
+    """Fused qkv rows -> normalised, rotated 16-bit heads in packed rows and / or cache slots
+    (sptmm_rotate_heads); device buffers, but inv_freq: one float64 per rotated channel pair, host
+    (None: no rotation)."""
+    f = np.ascontiguousarray(inv_freq, dtype=np.float64) if inv_freq is not None else np.empty(0)
+    p = _RotateParams(_ptr(QKV), _opt(q_norm), _opt(k_norm), f.ctypes.data if f.size else None, _opt(positions), _opt(slots),
+                      _ptr(Q), _opt(K), _opt(V), C.addressof(cache.struct) if cache is not None else None, ldqkv, ldq, ldk, ldv,
+                      T, heads, kv_heads, head_dim, in_dtype, dtype, 2 * f.size, 1 if interleaved else 0, eps)
+    check(lib.sptmm_rotate_heads(C.byref(p), flags, stream))
+
+
+def attention_prompt(Q, K, V, out, q_offsets, k_offsets, n_seqs: int, T: int, Tk: int, heads: int, kv_heads: int, head_dim: int,
+                     dtype: int = F16, causal: bool = True, scale: float = 0.0, ldq: int = 0, ldk: int = 0, ldv: int = 0, ldo: int = 0,
+                     flags: int = 0, stream: int = 0) -> None:
+    """Attention over packed sequences (sptmm_attention_prompt); device buffers, scale 0 = 1 / sqrt(head_dim)."""
+    p = _PromptParams(_ptr(Q), _opt(K), _opt(V), _ptr(out), _ptr(q_offsets), _ptr(k_offsets), ldq, ldk, ldv, ldo,
+                      n_seqs, T, Tk, heads, kv_heads, head_dim, dtype, 1 if causal else 0, scale)
+    check(lib.sptmm_attention_prompt(C.byref(p), flags, stream))
+
+
+def attention_decode_workspace(B: int, heads: int, kv_heads: int, head_dim: int, prefix_len: int = 0) -> int:
+    """Bytes of device workspace attention_decode needs."""
+    n = int(lib.sptmm_attention_decode_workspace(B, heads, kv_heads, head_dim, prefix_len))
+    if n == 0:
+        raise ValueError("attention_decode_workspace: " + lib.sptmm_last_error().decode("utf-8", "replace"))
+    return n
+
+
+def attention_decode(Q, out, B: int, heads: int, cache: KVCache, lengths, table, max_pages: int, prefix_table=None, prefix_len: int = 0,
+                     workspace=None, workspace_bytes: int = 0, scale: float = 0.0, ldq: int = 0, ldo: int = 0,
+                     flags: int = 0, stream: int = 0) -> None:
+    """One new token per sequence over a paged cache, behind an optional shared prefix (sptmm_attention_decode)."""
+    p = _DecodeParams(_ptr(Q), _ptr(out), C.addressof(cache.struct), _ptr(lengths), _opt(table), _opt(prefix_table), _opt(workspace),
+                      workspace_bytes, ldq, ldo, B, heads, max_pages, prefix_len, scale)
+    check(lib.sptmm_attention_decode(C.byref(p), flags, stream))
 
 
 def row_split3_small(X, W_pos_div, W_neg_div, out, M: int, K: int, N: int, S: int, split: int, stream: int = 0) -> None:
