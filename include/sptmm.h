@@ -566,6 +566,11 @@ typedef struct sptmm_decode_params {
 uint64_t sptmm_attention_decode_workspace(uint32_t B, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t prefix_len);
 int sptmm_attention_decode(const sptmm_decode_params *p, uint32_t flags, void *stream);
 
+/* The waits inside the attention kernels (on tile loads and tensor-core products) are bounded like
+ * those of the matmuls.  Waits for the current device and reads the word a wait that ran out raises
+ * there; 0 = every attention call since the last look completed normally. */
+int sptmm_attention_status(uint32_t *status);
+
 /* ---- small device helpers so a C caller needs no CUDA headers ------------------------------ */
 int sptmm_device_count(int *count);
 int sptmm_set_device(int device);

@@ -29,7 +29,7 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-r
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-pthread"]
 
 LIB_SOURCES = ["host_encode.cpp", "weights_file.cpp", "stack.cpp", "ternarise.cpp", "device_api.cu", "kernels_native.cu", "kernels_compat.cu", "kernels_seq.cu", "kernels_quant.cu", "kernels_rotate.cu", "kernels_prompt.cu", "kernels_decode.cu", "splitk.cu", "cublas_cmp.cu"]
-HEADERS = ["internal.h", "device_common.cuh", "attention.cuh", "tuning.h", os.path.join(ROOT, "include", "sptmm.h")]
+HEADERS = ["internal.h", "device_common.cuh", "attention.cuh", "tcgen05.cuh", "attention_tc.cuh", "tuning.h", os.path.join(ROOT, "include", "sptmm.h")]
 
 
 def _newer(target: str, deps: list[str]) -> bool:

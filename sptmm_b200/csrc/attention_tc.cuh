@@ -1,0 +1,503 @@
+// attention_tc.cuh -- the tensor-core attention kernel behind sptmm_attention_prompt (PREFIX false)
+// and behind the shared prefix of sptmm_attention_decode (PREFIX true).
+//
+//     O = softmax(scale * Q K^T) V
+//
+// A CTA owns two tiles of query rows of one key head and walks over the keys in blocks of 128 with the
+// running maximum m and sum l of the softmax, so scores never leave the SM.  A tile is 128 rows of
+// (token, query head of the group): all heads that share the keys share their tiles, and a short
+// sequence fills a tile with few tokens.  Per block and tile:
+//     S = Q K^T                  tcgen05, operands from shared memory, S (128 x 128 fp32) in tensor memory
+//     P = 2^(S scale - m)        one thread per row: m, l and the weights need no exchange between lanes
+//     O += P V                   tcgen05, P (16 bit) from tensor memory where S was, O in tensor memory
+// Warps: 0-3 the softmax of tile 0, 4-7 of tile 1, 8 the TMA loads (Q once, K and V blocks through a
+// ring), 9 issues the products, 10 looks for values that are not finite (below).  The products of one
+// tile run while the other tile is in its softmax; tensor memory is full: S0 S1 O0 O1 are 512 columns
+// at 128 channels.
+// When a row's maximum grows, O and l would have to be scaled down; that is put off until it has grown
+// by more than 2^8 (weights then stay below 2^8, harmless in fp32 sums and 16-bit weights alike, whose
+// relative rounding is the same), so after the first blocks it hardly ever happens.
+// Masks: keys a row does not see get the score -inf before the maximum, blocks nobody sees are not
+// visited, values behind the last visible key are overwritten with zeros in shared memory (a weight of
+// zero times another sequence's NaN would be NaN).  Values that SOME rows of the CTA see (the causal
+// diagonal) must stay; should one of them be NaN or infinite, warp 10 finds it and the CTA's rows are
+// computed once more row by row (attend_row), where hidden keys are not touched at all.
+#pragma once
+#include "tcgen05.cuh"
+
+namespace sptmm {
+
+struct TcParams {
+    const void *Q, *K, *V;
+    void *O;
+    const int32_t *q_off, *k_off;            // prompt
+    uint64_t ldq, ldk, ldv, ldo;
+    uint32_t n_seqs, T, Tk, heads, kv_heads, group, head_dim, causal;
+    uint32_t tokens;                         // tokens per tile, 128 / group
+    float scale;                             // scale * log2(e)
+    // the shared prefix of a decode step: keys in pages, parts of the keys in different CTAs
+    const int32_t *prefix_table;
+    uint32_t prefix_len, n_pages, page_shift, splits, blocks_per_split;
+    float *part_o;                           // [token][head][split][head_dim], not divided by l
+    float2 *part_ml;                         // [token][head][split]: (m in powers of two, l)
+    uint32_t *status;
+};
+
+constexpr uint32_t kTcThreads = 352;
+constexpr uint32_t kKeys = 128;              // keys per block
+
+template <int DP> struct TcLayout {
+    static constexpr uint32_t slabs = DP / 64, tile = 128 * DP * 2;
+    static constexpr uint32_t stages = DP == 128 ? 5 : 8;
+    static constexpr uint32_t smem = 2 * tile + stages * tile + 1024;      // 1024: room to align
+};
+
+// One row by CUDA cores: a warp, four channels per lane, keys k0 .. k0 + n one after the other.
+template <typename T>
+__device__ void attend_row(const TcParams &p, uint32_t t, uint32_t h, uint32_t kh, uint32_t k0, uint32_t n)
+{
+    const uint32_t lane = threadIdx.x & 31, c = lane * 4, D = p.head_dim;
+    float q[4] = {0, 0, 0, 0}, o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0;
+    if (c < D) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const T *>(p.Q) + (uint64_t)t * p.ldq + (uint64_t)h * D + c);
+        const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
+        q[0] = a.x * p.scale; q[1] = a.y * p.scale; q[2] = b.x * p.scale; q[3] = b.y * p.scale;
+    }
+    for (uint32_t j = 0; j < n; j++) {
+        float k[4] = {0, 0, 0, 0}, v[4] = {0, 0, 0, 0};
+        if (c < D) {
+            const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const T *>(p.K) + (uint64_t)(k0 + j) * p.ldk + (uint64_t)kh * D + c);
+            const uint2 z = *reinterpret_cast<const uint2 *>(static_cast<const T *>(p.V) + (uint64_t)(k0 + j) * p.ldv + (uint64_t)kh * D + c);
+            float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
+            k[0] = a.x; k[1] = a.y; k[2] = b.x; k[3] = b.y;
+            a = unpack2<T>(z.x); b = unpack2<T>(z.y);
+            v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+        }
+        float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
+#pragma unroll
+        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+        const float m1 = fmaxf(m, s), base = m1 == -INFINITY ? 0.0f : m1;
+        const float w0 = ex2(m - base), w1 = ex2(s - base);
+        m = m1;
+        l = l * w0 + w1;
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = o[i] * w0 + w1 * v[i];
+    }
+    if (c >= D) return;
+    const float r = l == 0.0f ? 0.0f : 1.0f / l;
+    *reinterpret_cast<uint2 *>(static_cast<T *>(p.O) + (uint64_t)t * p.ldo + (uint64_t)h * D + c) =
+        make_uint2(pack2<T>(o[0] * r, o[1] * r), pack2<T>(o[2] * r, o[3] * r));
+}
+
+// What a CTA works on.  Query i of the sequence (0 .. n_q) is row q0 + i and sees keys 0 .. i + shift of
+// the m keys from row k0, at most m.
+struct TcItem {
+    uint32_t q0, n_q, k0, m, first;          // `first`: the CTA's first query
+    int32_t shift;                           // causal: m - n_q; else so large that every query sees all
+    uint32_t block0, blocks;                 // blocks of 128 keys
+    bool any;
+    __device__ __forceinline__ uint32_t visible(uint32_t i) const
+    {
+        const int64_t v = (int64_t)i + shift + 1;
+        return v < 0 ? 0u : (uint32_t)min(v, (int64_t)m);
+    }
+};
+
+__device__ __forceinline__ void seq_range(const TcParams &p, uint32_t s, uint32_t &q0, uint32_t &n, uint32_t &k0, uint32_t &m)
+{
+    const int32_t a = min(max(p.q_off[s], 0), (int32_t)p.T), b = min(max(p.q_off[s + 1], a), (int32_t)p.T);
+    const int32_t c = min(max(p.k_off[s], 0), (int32_t)p.Tk), d = min(max(p.k_off[s + 1], c), (int32_t)p.Tk);
+    q0 = a; n = b - a; k0 = c; m = d - c;
+}
+
+// Items (pairs of tiles) in falling order of the keys they visit, so that the longest start first and
+// the short ones fill the end.  An item's level is the number of its pair of tiles counted from the
+// sequence's first key; rank `w` is looked up by counting the items at or above a level (a warp, lanes
+// over sequences).
+__device__ __forceinline__ bool find_item(const TcParams &p, uint32_t w, uint32_t &seq, uint32_t &pair)
+{
+    const uint32_t lane = threadIdx.x & 31, per = 2 * p.tokens;
+    // items and first level of sequence s
+    auto shape = [&](uint32_t s, uint32_t &n, uint32_t &low) {
+        uint32_t q0, nq, k0, m;
+        seq_range(p, s, q0, nq, k0, m);
+        n = (nq + per - 1) / per;
+        low = p.causal ? (m > nq ? (m - nq) / per : 0u) : m / per;
+    };
+    auto at_or_above = [&](uint32_t n, uint32_t low, uint32_t x) -> uint32_t {
+        if (!p.causal) return low >= x ? n : 0u;
+        return x <= low ? n : (x - low >= n ? 0u : n - (x - low));
+    };
+    uint32_t n1 = 0, low1 = 0;               // the first 32 sequences stay in registers
+    if (lane < p.n_seqs) shape(lane, n1, low1);
+    uint32_t top = n1 + low1, total = n1;
+    for (uint32_t s = lane + 32; s < p.n_seqs; s += 32) {
+        uint32_t n, low;
+        shape(s, n, low);
+        top = max(top, n + low); total += n;
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    if (w >= total) return false;
+    auto count = [&](uint32_t x) {
+        uint32_t c = at_or_above(n1, low1, x);
+        for (uint32_t s = lane + 32; s < p.n_seqs; s += 32) {
+            uint32_t n, low;
+            shape(s, n, low);
+            c += at_or_above(n, low, x);
+        }
+        return __reduce_add_sync(0xffffffffu, c);
+    };
+    uint32_t lo = 0, hi = __reduce_max_sync(0xffffffffu, top) + 1;          // count(lo) > w, count(hi) <= w
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (count(mid) > w) lo = mid; else hi = mid;
+    }
+    uint32_t left = w - count(lo + 1);       // among the items of level lo, in order of sequences
+    for (uint32_t s0 = 0; s0 < p.n_seqs; s0 += 32) {
+        const uint32_t s = s0 + lane;
+        uint32_t n = n1, low = low1;
+        if (s0) { n = low = 0; if (s < p.n_seqs) shape(s, n, low); }
+        const uint32_t here = at_or_above(n, low, lo) - at_or_above(n, low, lo + 1);
+        uint32_t sum = here;                 // inclusive prefix over the lanes
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= (uint32_t)o) sum += y;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, left < sum);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            const uint32_t before = sum - here, pr = p.causal ? lo - low : left - before;
+            seq = s0 + src;
+            pair = __shfl_sync(0xffffffffu, pr, src);
+            return true;
+        }
+        left -= __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return false;
+}
+
+template <typename T, int DP, bool PREFIX>
+__global__ void __launch_bounds__(kTcThreads, 1)
+k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+               const __grid_constant__ CUtensorMap map_v)
+{
+    using L = TcLayout<DP>;
+    constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
+    extern __shared__ unsigned char dyn[];
+    __shared__ uint64_t bars[2 + 2 * L::stages + 2 + 2 + 2 + 1 + 1];
+    __shared__ uint32_t tmem_base, abort_flag, bad_values, item_seq, item_pair, item_ok;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t bar0 = smem_addr(bars);
+    const uint32_t b_q = bar0, b_full = bar0 + 16, b_empty = b_full + 8 * L::stages, b_s = b_empty + 8 * L::stages, b_p = b_s + 16,
+                   b_o = b_p + 16, b_fix = b_o + 16, b_end = b_fix + 8;
+    volatile uint32_t *abort_word = &abort_flag;
+    pdl_launch_dependents();
+    if (warp == 8) {
+        if (lane == 0) {
+            mbar_init(b_q, 1); mbar_init(b_q + 8, 1);
+            for (uint32_t i = 0; i < L::stages; i++) { mbar_init(b_full + 8 * i, 1); mbar_init(b_empty + 8 * i, 1); }
+            for (uint32_t t = 0; t < 2; t++) { mbar_init(b_s + 8 * t, 1); mbar_init(b_p + 8 * t, 4); mbar_init(b_o + 8 * t, 1); }
+            mbar_init(b_fix, 1); mbar_init(b_end, 1);
+            abort_flag = 0; bad_values = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            tma_prefetch_map(&map_q); tma_prefetch_map(&map_k); tma_prefetch_map(&map_v);
+        }
+    } else if (warp == 9) {
+        tmem_alloc(smem_addr(&tmem_base), 512);
+    }
+    pdl_wait_prior_grid();
+    uint32_t kh, split = 0;
+    if constexpr (PREFIX) {
+        split = blockIdx.x % p.splits;
+        kh = blockIdx.x / p.splits % p.kv_heads;
+    } else {
+        kh = blockIdx.x % p.kv_heads;
+        if (warp == 0) {
+            uint32_t s = 0, pr = 0;
+            const bool ok = find_item(p, blockIdx.x / p.kv_heads, s, pr);
+            if (lane == 0) { item_ok = ok; item_seq = s; item_pair = pr; }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    TcItem it;
+    if constexpr (PREFIX) {
+        it.q0 = 0; it.n_q = p.T; it.k0 = 0; it.m = p.prefix_len; it.shift = (int32_t)p.prefix_len;
+        it.first = blockIdx.x / p.splits / p.kv_heads * 2 * p.tokens;
+        it.any = true;
+        it.block0 = split * p.blocks_per_split;
+        it.blocks = min((p.prefix_len + kKeys - 1) / kKeys, it.block0 + p.blocks_per_split) - it.block0;
+    } else {
+        it.any = item_ok;
+        seq_range(p, it.any ? item_seq : 0, it.q0, it.n_q, it.k0, it.m);
+        it.shift = p.causal ? (int32_t)it.m - (int32_t)it.n_q : 0x40000000;
+        it.first = (it.any ? item_pair : 0) * 2 * p.tokens;
+        it.block0 = 0;
+        it.blocks = it.any ? (it.visible(min(it.n_q, it.first + 2 * p.tokens) - 1) + kKeys - 1) / kKeys : 0;
+    }
+    const uint32_t n_here = it.any ? min(it.n_q - it.first, 2 * p.tokens) : 0;      // queries of this CTA
+    const uint32_t n_tiles = n_here > p.tokens ? 2 : 1;
+    const uint32_t last_key = it.any ? it.visible(it.first + n_here - 1) : 0;       // keys nobody here sees start at this one
+    const uint32_t q_smem = (smem_addr(dyn) + 1023) & ~1023u, ring = q_smem + 2 * L::tile;
+    const uint32_t tmem = tmem_base;
+    const uint32_t n = it.blocks;
+    const uint32_t D = p.head_dim, slabs = (D + 63) / 64;
+    uint32_t issued = 0;                     // ring loads on their way (the loading thread's)
+    const bool cut = (it.block0 + n) * kKeys > last_key;                            // the last block holds keys nobody sees
+
+    if (warp < 8) {
+        // ---- softmax: thread = row --------------------------------------------------------------
+        const uint32_t tile = warp >> 2, row = tid & 127, s_addr = tmem + tile * 128 + ((warp & 3) << 21), o_addr = tmem + 256 + tile * DP + ((warp & 3) << 21);
+        const uint32_t tok = tile * p.tokens + row / p.group, head = kh * p.group + row % p.group;      // row / group < tokens for rows in use
+        const bool mine = row < p.tokens * p.group && tok < n_here;
+        const uint32_t vis = mine ? it.visible(it.first + tok) : it.m;         // rows not in use are never stored: no mask for their sake
+        float m = -INFINITY, l = 0.0f;       // m in units of the raw score
+        const float sc = p.scale;
+        bool ok = true;
+        if (tile < n_tiles && n > 0) {
+            for (uint32_t i = 0; i < n; i++) {
+                const uint32_t j0 = (it.block0 + i) * kKeys;
+                uint32_t pages_ok = 0xffu;
+                if constexpr (PREFIX) {                                             // which pages of the block lie in the cache
+                    const uint32_t per = kKeys >> p.page_shift, at = (j0 >> p.page_shift) + lane;
+                    bool good = true;
+                    if (lane < per && (at << p.page_shift) < p.prefix_len) good = (uint32_t)p.prefix_table[at] < p.n_pages;
+                    pages_ok = __ballot_sync(0xffffffffu, good);
+                }
+                if (!mbar_wait(b_s + 8 * tile, i & 1, abort_word)) ok = false;
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                tc_fence_after();
+                uint32_t r[128];
+#pragma unroll
+                for (int c = 0; c < 4; c++) tmem_ld32(s_addr + 32 * c, r + 32 * c);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 4; c++) pin32(r + 32 * c);
+                if (__any_sync(0xffffffffu, j0 + kKeys > vis)) {
+                    const int32_t left = (int32_t)vis - (int32_t)j0;
+#pragma unroll
+                    for (int c = 0; c < 128; c++) if (c >= left) r[c] = 0xff800000u;
+                }
+                if constexpr (PREFIX) {
+                    if ((pages_ok & 0xffu) != 0xffu)
+#pragma unroll
+                        for (int c = 0; c < 128; c++) if (!(pages_ok >> (c >> p.page_shift) & 1)) r[c] = 0xff800000u;
+                }
+                float mx[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) mx[c] = fmaxf(__uint_as_float(r[c]), __uint_as_float(r[c + 4]));
+#pragma unroll
+                for (int c = 8; c < 128; c += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], __uint_as_float(r[c + e]), __uint_as_float(r[c + 4 + e]));
+                const float mb = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                // a first finite maximum, or one more than 2^8 above the one in use: scale O and l
+                const bool grow = mine && mb > m && (m == -INFINITY || (mb - m) * sc > 8.0f);
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float m1 = fmaxf(m, mb), w = m == -INFINITY ? (m1 == -INFINITY ? 1.0f : 0.0f) : ex2((m - m1) * sc);
+                    m = m1;
+                    l *= w;
+                    if (i > 0) {
+                        for (uint32_t c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(o_addr + c, o);
+                            tmem_wait_ld();
+                            pin32(o);
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * w);
+                            tmem_st32(o_addr + c, o);
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.0f : m * sc;
+                const uint64_t sc2 = f2_pack(sc, sc), nb2 = f2_pack(-base, -base);
+                uint64_t sum[2] = {0, 0};
+                uint32_t w[64];
+#pragma unroll
+                for (int c = 0; c < 128; c += 2) {
+                    const float2 x = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sc2, nb2));
+                    const float a = ex2(x.x), b = ex2(x.y);
+                    sum[(c >> 1) & 1] = f2_add(sum[(c >> 1) & 1], f2_pack(a, b));
+                    w[c >> 1] = pack2<T>(a, b);
+                }
+                tmem_st32(s_addr, w);
+                tmem_st32(s_addr + 32, w + 32);
+                const float2 z = f2_unpack(f2_add(sum[0], sum[1]));
+                l += z.x + z.y;
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(b_p + 8 * tile);
+            }
+            if (ok && !mbar_wait(b_o + 8 * tile, 0, abort_word)) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+        }
+        // ---- epilogue ----
+        if (ok && tile < n_tiles) {
+            if constexpr (PREFIX) {
+                const uint64_t at = ((uint64_t)(it.first + tok) * p.heads + head) * p.splits + split;
+                if (mine) p.part_ml[at] = make_float2(m == -INFINITY ? -INFINITY : m * sc, l);
+                for (uint32_t c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(o_addr + c, o);
+                    tmem_wait_ld();
+                    pin32(o);
+                    if (mine)
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            if (c + e < D) *reinterpret_cast<uint4 *>(p.part_o + at * D + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+            } else {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                T *out = static_cast<T *>(p.O) + (uint64_t)(it.q0 + it.first + tok) * p.ldo + (uint64_t)head * D;
+                for (uint32_t c = 0; c < D; c += 32) {
+                    uint32_t o[32] = {};
+                    if (n > 0) {
+                        tmem_ld32(o_addr + c, o);
+                        tmem_wait_ld();
+                        pin32(o);
+                    }
+                    if (mine)
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8)
+                            if (c + e < D) {
+                                uint32_t y[4];
+#pragma unroll
+                                for (int x = 0; x < 4; x++)
+                                    y[x] = vis == 0 ? 0u : pack2<T>(__uint_as_float(o[e + 2 * x]) * inv, __uint_as_float(o[e + 2 * x + 1]) * inv);
+                                *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(y[0], y[1], y[2], y[3]);
+                            }
+                }
+            }
+        }
+    } else if (warp == 8) {
+        // ---- loads -------------------------------------------------------------------------------
+        bool ok = true;
+        const uint32_t group = p.group;
+        if (lane == 0 && n > 0) {
+            for (uint32_t t = 0; t < n_tiles; t++) {
+                mbar_expect(b_q + 8 * t, slabs * p.tokens * group * 128);
+                for (uint32_t s = 0; s < slabs; s++)
+                    tma_load_3d(q_smem + t * L::tile + s * 16384, &map_q, b_q + 8 * t, s * 64, kh * group, it.q0 + it.first + t * p.tokens);
+            }
+            for (uint32_t x = 0; x < 2 * n && ok; x++) {                            // K0 V0 K1 V1 ...
+                const uint32_t st = x % L::stages, use = x / L::stages, i = x >> 1;
+                if (use > 0 && !mbar_wait(b_empty + 8 * st, (use - 1) & 1, abort_word)) { ok = false; break; }
+                issued = x + 1;
+                const CUtensorMap *map = x & 1 ? &map_v : &map_k;
+                const uint32_t dst = ring + st * L::tile, bar = b_full + 8 * st, j0 = (it.block0 + i) * kKeys;
+                if constexpr (PREFIX) {
+                    const uint32_t size = 1u << p.page_shift, keys = min(kKeys, p.prefix_len - j0), pages = (keys + size - 1) >> p.page_shift;
+                    mbar_expect(bar, slabs * pages * size * 128);
+                    for (uint32_t g = 0; g < pages; g++) {
+                        const uint32_t page = (uint32_t)p.prefix_table[(j0 >> p.page_shift) + g];
+                        const int32_t at = page < p.n_pages ? (int32_t)page : (int32_t)p.n_pages;       // outside the cache: reads as zeros
+                        for (uint32_t s = 0; s < slabs; s++) tma_load_4d(dst + s * 16384 + g * size * 128, map, bar, s * 64, 0, kh, at);
+                    }
+                } else {
+                    mbar_expect(bar, slabs * 16384);
+                    for (uint32_t s = 0; s < slabs; s++) tma_load_3d(dst + s * 16384, map, bar, s * 64, kh, it.k0 + j0);
+                }
+            }
+        }
+        ok = __shfl_sync(0xffffffffu, (uint32_t)ok, 0);
+        // zeros over the values that nobody here sees
+        if (ok && n > 0 && cut) {
+            const uint32_t x = 2 * n - 1, st = x % L::stages;
+            if (mbar_wait(b_full + 8 * st, x / L::stages & 1, abort_word)) {
+                const uint32_t from = last_key - (it.block0 + n - 1) * kKeys;
+                for (uint32_t s = 0; s < slabs; s++)
+                    for (uint32_t a = from * 128 + lane * 16; a < 16384; a += 512)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ring + st * L::tile + s * 16384 + a), "r"(0u) : "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(b_fix);
+            }
+        }
+    } else if (warp == 9) {
+        // ---- products ----------------------------------------------------------------------------
+        if (lane == 0 && n > 0) {
+            const uint32_t steps = (D + 15) / 16;
+            const uint32_t desc_s = mma_desc(kBf16, 128, false), desc_o = mma_desc(kBf16, steps * 16, true);
+            bool ok = true;
+            auto scores = [&](uint32_t t, uint32_t x) {                              // S_t = Q_t K^T, K in ring use x
+                const uint32_t kb = ring + x % L::stages * L::tile, qb = q_smem + t * L::tile;
+                for (uint32_t k = 0; k < steps; k++) {
+                    const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
+                    mma_ss(tmem + t * 128, smem_desc(qb + off, 0, 1024), smem_desc(kb + off, 0, 1024), desc_s, k > 0);
+                }
+                tc_commit(b_s + 8 * t);
+            };
+            auto full = [&](uint32_t x) { return mbar_wait(b_full + 8 * (x % L::stages), x / L::stages & 1, abort_word); };
+            ok = full(0);
+            for (uint32_t t = 0; t < n_tiles && ok; t++) {
+                ok = mbar_wait(b_q + 8 * t, 0, abort_word);
+                if (ok) { tc_fence_after(); scores(t, 0); }
+            }
+            if (ok) tc_commit(b_empty);
+            for (uint32_t i = 0; i < n && ok; i++) {
+                const bool last = i + 1 == n;
+                ok = full(2 * i + 1) && (last || full(2 * i + 2)) && (!last || !cut || mbar_wait(b_fix, 0, abort_word));
+                const uint32_t vb = ring + (2 * i + 1) % L::stages * L::tile;
+                for (uint32_t t = 0; t < n_tiles && ok; t++) {
+                    ok = mbar_wait(b_p + 8 * t, i & 1, abort_word);
+                    if (!ok) break;
+                    tc_fence_after();
+                    for (uint32_t k = 0; k < 8; k++)                                 // O_t += P_t V, sixteen keys at a time
+                        mma_ts(tmem + 256 + t * DP, tmem + t * 128 + k * 8, smem_desc(vb + k * 2048, 16384, 1024), desc_o, i > 0 || k > 0);
+                    if (!last) scores(t, 2 * i + 2);
+                    else tc_commit(b_o + 8 * t);
+                }
+                if (ok) {
+                    tc_commit(b_empty + 8 * ((2 * i + 1) % L::stages));
+                    if (!last) tc_commit(b_empty + 8 * ((2 * i + 2) % L::stages));
+                }
+            }
+        }
+    } else if (!PREFIX && n > 0 && p.causal) {
+        // ---- values that some rows here see and others do not: all finite? --------------------------
+        const uint32_t from = it.visible(it.first);
+        uint32_t found = 0;
+        const uint32_t per = D / 8;                                                  // 16-byte words per row
+        for (uint32_t x = lane; x < (last_key - from) * per; x += 32) {
+            const uint32_t j = from + x / per, c = x % per * 8;
+            const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.V) + (uint64_t)(it.k0 + j) * p.ldv + (uint64_t)kh * D + c);
+            constexpr uint32_t e = kBf16 ? 0x7f807f80u : 0x7c007c00u;                // exponent bits; all set in a half: not finite
+            for (uint32_t y : {v.x, v.y, v.z, v.w}) {
+                const uint32_t b = y & e;
+                if ((b & 0xffffu) == (e & 0xffffu) || (b >> 16) == (e >> 16)) found = 1;
+            }
+        }
+        if (__any_sync(0xffffffffu, found) && lane == 0) bad_values = 1;
+    }
+    __syncwarp();
+    __syncthreads();
+    if (abort_flag) {
+        // a wait ran out (never in a healthy run): report, then let copies and products in flight end
+        if (tid == 0) atomicOr(p.status, 1u);
+        uint32_t never = 0;
+        if (tid == 9 * 32 && n > 0) {
+            tc_commit(b_end);                // arrives when every product issued so far is done
+            mbar_wait(b_end, 0, &never);
+        }
+        if (tid == 8 * 32 && n > 0) {
+            for (uint32_t t = 0; t < n_tiles; t++) mbar_wait(b_q + 8 * t, 0, &never);
+            for (uint32_t x = issued > L::stages ? issued - L::stages : 0; x < issued; x++) mbar_wait(b_full + 8 * (x % L::stages), x / L::stages & 1, &never);
+        }
+        __syncthreads();
+    } else if (!PREFIX && bad_values) {
+        for (uint32_t x = warp; x < n_here * p.group; x += kTcThreads / 32) {
+            const uint32_t i = it.first + x / p.group;
+            attend_row<T>(p, it.q0 + i, kh * p.group + x % p.group, kh, it.k0, it.visible(i));
+        }
+    }
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_free(tmem, 512);
+    }
+}
+
+}  // namespace sptmm

@@ -1,69 +1,52 @@
 // kernels_prompt.cu -- attention over packed prompts.
 //
 // The reference has no attention (its only operator is the matmul, main.cu:993-1961).
-// Simplest form: a warp per (query row, head), four channels per lane, keys one after the other with
-// the running maximum and sum of the softmax in fp32.
-#include "attention.cuh"
+// The kernel is k_attention_tc (attention_tc.cuh); here are its host side, the tensor maps and the word
+// an expired wait is reported in.
+#include <atomic>
+
+#include "attention_tc.cuh"
 
 namespace sptmm {
 
-struct PromptParams {
-    const void *Q, *K, *V;
-    void *O;
-    const int32_t *q_off, *k_off;
-    uint64_t ldq, ldk, ldv, ldo;
-    uint32_t n_seqs, T, Tk, heads, group, head_dim, causal;
-    float scale;
-};
+__device__ uint32_t g_attention_status;
 
-template <typename T>
-__global__ void __launch_bounds__(256) k_prompt_rows(const PromptParams p)
+int attention_status_word(uint32_t **dev_word)
 {
-    const uint32_t lane = threadIdx.x & 31, c = lane * 4, D = p.head_dim;
-    const uint64_t item = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    pdl_launch_dependents();
-    pdl_wait_prior_grid();
-    if (item >= (uint64_t)p.T * p.heads) return;
-    const uint32_t t = (uint32_t)(item / p.heads), h = (uint32_t)(item % p.heads), kh = h / p.group;
-    uint32_t lo = 0, hi = p.n_seqs;                          // the last sequence that starts at or before t
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (p.q_off[mid] <= (int32_t)t) lo = mid; else hi = mid;
+    SPTMM_CUDA_TRY(cudaGetSymbolAddress(reinterpret_cast<void **>(dev_word), g_attention_status));
+    return SPTMM_OK;
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+int make_tensor_map(const char *who, CUtensorMap *map, const void *base, uint32_t dtype, uint32_t rank, const uint64_t *dims,
+                    const uint64_t *strides, const uint32_t *box)
+{
+    static std::atomic<void *> entry{nullptr};       // the driver's function; the same whoever looks it up first
+    void *fn = entry.load();
+    if (!fn) {
+        cudaDriverEntryPointQueryResult found;
+        SPTMM_CUDA_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
+        if (found != cudaDriverEntryPointSuccess || !fn) return fail(SPTMM_ERR_CUDA, "%s: the driver has no tensor maps", who);
+        entry.store(fn);
     }
-    const int32_t q0 = max(p.q_off[lo], 0), q1 = min(p.q_off[lo + 1], (int32_t)p.T);        // offsets past the rows are cut
-    if ((int32_t)t < q0 || (int32_t)t >= q1) return;
-    const int32_t k0 = max(p.k_off[lo], 0), k1 = max(k0, min(p.k_off[lo + 1], (int32_t)p.Tk));
-    int64_t n = k1 - k0;
-    if (p.causal) n = min(n, max((int64_t)0, (int64_t)(t - q0) + n - (q1 - q0) + 1));
-    float q[4] = {0, 0, 0, 0}, o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0;
-    if (c < D) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const T *>(p.Q) + (uint64_t)t * p.ldq + (uint64_t)h * D + c);
-        const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
-        q[0] = a.x * p.scale; q[1] = a.y * p.scale; q[2] = b.x * p.scale; q[3] = b.y * p.scale;
-    }
-    for (int64_t j = 0; j < n; j++) {
-        float k[4] = {0, 0, 0, 0}, v[4] = {0, 0, 0, 0};
-        if (c < D) {
-            const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const T *>(p.K) + (uint64_t)(k0 + j) * p.ldk + (uint64_t)kh * D + c);
-            const uint2 z = *reinterpret_cast<const uint2 *>(static_cast<const T *>(p.V) + (uint64_t)(k0 + j) * p.ldv + (uint64_t)kh * D + c);
-            float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
-            k[0] = a.x; k[1] = a.y; k[2] = b.x; k[3] = b.y;
-            a = unpack2<T>(z.x); b = unpack2<T>(z.y);
-            v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
-        }
-        float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
-#pragma unroll
-        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        const float m1 = fmaxf(m, s), w0 = m1 == -INFINITY ? 1.0f : exp2f(m - m1), w1 = m1 == -INFINITY ? 0.0f : exp2f(s - m1);
-        m = m1;
-        l = l * w0 + w1;
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = o[i] * w0 + w1 * v[i];
-    }
-    if (c >= D) return;
-    const float r = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-    *reinterpret_cast<uint2 *>(static_cast<T *>(p.O) + (uint64_t)t * p.ldo + (uint64_t)h * D + c) =
-        make_uint2(pack2<T>(o[0] * r, o[1] * r), pack2<T>(o[2] * r, o[3] * r));
+    cuuint64_t d[4], st[3];
+    cuuint32_t b[4], one[4];
+    for (uint32_t i = 0; i < rank; i++) { d[i] = dims[i]; b[i] = box[i]; one[i] = 1; if (i) st[i - 1] = strides[i - 1]; }
+    const CUresult rc = reinterpret_cast<EncodeTiled>(fn)(map, dtype == SPTMM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                                          rank, const_cast<void *>(base), d, st, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return fail(SPTMM_ERR_CUDA, "%s: tensor map refused (%d)", who, (int)rc);
+    return SPTMM_OK;
+}
+
+template <typename T, int DP>
+static cudaError_t launch_prompt(const TcParams &prm, uint32_t grid, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, void *stream, bool pdl)
+{
+    const cudaError_t e = cudaFuncSetAttribute(k_attention_tc<T, DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<DP>::smem);
+    if (e != cudaSuccess) return e;
+    return launch(k_attention_tc<T, DP, false>, dim3(grid), dim3(kTcThreads), TcLayout<DP>::smem, stream, pdl, prm, q, k, v);
 }
 
 }  // namespace sptmm
@@ -78,7 +61,7 @@ extern "C" int sptmm_attention_prompt(const sptmm_prompt_params *a, uint32_t fla
     if (rc != SPTMM_OK) return rc;
     if (flags & ~(uint32_t)SPTMM_LAUNCH_PDL) return fail(SPTMM_ERR_INVALID, "%s: flags %u", who, flags);
     if (!(a->scale >= 0.0f) || a->scale > 1e30f) return fail(SPTMM_ERR_INVALID, "%s: scale %g", who, (double)a->scale);
-    PromptParams prm{};
+    TcParams prm{};
     prm.ldq = a->ldq; prm.ldk = a->ldk; prm.ldv = a->ldv; prm.ldo = a->ldo;
     const uint64_t q_width = (uint64_t)a->heads * a->head_dim, kv_width = (uint64_t)a->kv_heads * a->head_dim;
     rc = check_stride(who, "ldq", prm.ldq, q_width, 8);
@@ -93,14 +76,41 @@ extern "C" int sptmm_attention_prompt(const sptmm_prompt_params *a, uint32_t fla
     for (const void *x : {a->Q, a->K, a->V, (const void *)a->O})
         if (!aligned16(x)) return fail(SPTMM_ERR_INVALID, "%s: an address is not 16-byte aligned", who);
     prm.Q = a->Q; prm.K = a->K; prm.V = a->V; prm.O = a->O; prm.q_off = a->q_offsets; prm.k_off = a->k_offsets;
-    prm.n_seqs = a->n_seqs; prm.T = a->T; prm.Tk = a->Tk; prm.heads = a->heads; prm.group = a->heads / a->kv_heads;
+    prm.n_seqs = a->n_seqs; prm.T = a->T; prm.Tk = a->Tk; prm.heads = a->heads; prm.kv_heads = a->kv_heads; prm.group = a->heads / a->kv_heads;
     prm.head_dim = a->head_dim; prm.causal = a->causal ? 1 : 0;
+    prm.tokens = 128 / prm.group;
     prm.scale = (a->scale > 0.0f ? a->scale : 1.0f / sqrtf((float)a->head_dim)) * 1.4426950408889634f;     // log2(e): the kernel works with exp2
-    const uint64_t warps = (uint64_t)a->T * a->heads;
-    if (warps > 0x7fffffffull * 8) return fail(SPTMM_ERR_UNSUPPORTED, "%s: %u rows of %u heads in one call", who, a->T, a->heads);
-    const dim3 grid((uint32_t)((warps + 7) / 8));
-    const cudaError_t e = a->dtype == SPTMM_F16 ? launch(k_prompt_rows<__half>, grid, dim3(256), 0, stream, flags & SPTMM_LAUNCH_PDL, prm)
-                                                : launch(k_prompt_rows<__nv_bfloat16>, grid, dim3(256), 0, stream, flags & SPTMM_LAUNCH_PDL, prm);
+    // pairs of tiles: every sequence may end with a part of one
+    const uint64_t items = (uint64_t)a->T / (2 * prm.tokens) + (a->n_seqs < a->T ? a->n_seqs : a->T);
+    if (items * a->kv_heads > 0x7fffffffull) return fail(SPTMM_ERR_UNSUPPORTED, "%s: %u rows of %u key heads in one call", who, a->T, a->kv_heads);
+    rc = attention_status_word(&prm.status);
+    if (rc != SPTMM_OK) return rc;
+    const uint64_t D = a->head_dim, es = 2;
+    const uint64_t dims_q[3] = {D, a->heads, a->T}, str_q[2] = {D * es, prm.ldq * es};
+    const uint64_t dims_k[3] = {D, a->kv_heads, a->Tk ? a->Tk : 1}, str_k[2] = {D * es, prm.ldk * es}, str_v[2] = {D * es, prm.ldv * es};
+    const uint32_t box_q[3] = {64, prm.group, prm.tokens}, box_k[3] = {64, 1, kKeys};
+    CUtensorMap mq, mk, mv;
+    rc = make_tensor_map(who, &mq, a->Q, a->dtype, 3, dims_q, str_q, box_q);
+    if (rc == SPTMM_OK) rc = make_tensor_map(who, &mk, a->Tk ? a->K : a->Q, a->dtype, 3, dims_k, str_k, box_k);     // no keys: never read
+    if (rc == SPTMM_OK) rc = make_tensor_map(who, &mv, a->Tk ? a->V : a->Q, a->dtype, 3, dims_k, str_v, box_k);
+    if (rc != SPTMM_OK) return rc;
+    const uint32_t grid = (uint32_t)(items * a->kv_heads);
+    const bool pdl = flags & SPTMM_LAUNCH_PDL, wide = a->head_dim > 64;
+    cudaError_t e;
+    if (a->dtype == SPTMM_F16) e = wide ? launch_prompt<__half, 128>(prm, grid, mq, mk, mv, stream, pdl) : launch_prompt<__half, 64>(prm, grid, mq, mk, mv, stream, pdl);
+    else e = wide ? launch_prompt<__nv_bfloat16, 128>(prm, grid, mq, mk, mv, stream, pdl) : launch_prompt<__nv_bfloat16, 64>(prm, grid, mq, mk, mv, stream, pdl);
     if (e != cudaSuccess) return fail(SPTMM_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+    return SPTMM_OK;
+}
+
+extern "C" int sptmm_attention_status(uint32_t *status)
+{
+    if (!status) return fail(SPTMM_ERR_INVALID, "attention_status: null pointer");
+    SPTMM_CUDA_TRY(cudaDeviceSynchronize());
+    SPTMM_CUDA_TRY(cudaMemcpyFromSymbol(status, g_attention_status, sizeof(uint32_t)));
+    if (*status) {
+        const uint32_t zero = 0;
+        SPTMM_CUDA_TRY(cudaMemcpyToSymbol(g_attention_status, &zero, sizeof zero));
+    }
     return SPTMM_OK;
 }
