@@ -1,69 +1,400 @@
 // kernels_decode.cu -- attention of one new token per sequence over a paged cache, behind an optional
 // prefix that the batch shares.
 //
-// The reference has no attention (its only operator is the matmul, main.cu:993-1961).
-// Simplest form: a warp per (sequence, head), four channels per lane, keys one after the other.
-#include "attention.cuh"
+// The reference has no attention (its only operator is the matmul, main.cu:993-1961).  HBM bound: a key
+// and its value are read once and used for the query heads that share them.  Three kernels, launched
+// with programmatic overlap:
+//   k_attention_tc<.., true>   (only with a prefix) all rows of the batch against the prefix, each part
+//                              of its keys in another CTA; see attention_tc.cuh
+//   k_decode                   every sequence's own keys
+//   k_decode_join              the parts of a row -> one softmax: with parts (m_i, l_i, o_i) and M = max m_i,
+//                              O = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i
+// k_decode splits the work by keys, not by sequences: all (sequence, key head) units are laid end to end
+// in blocks of 64 keys and every CTA takes an equal run of blocks, wherever sequences begin and end in
+// it, so that one sequence of 128k tokens fills the GPU as well as 64 of different lengths do.  The
+// lengths are read on the device.  Unit u's piece in CTA c is number u + c: along the walk either u or c
+// grows, so numbers are unique and a unit's pieces are neighbours.
+// Within a CTA each of four warps takes 16 keys of a block for itself: K and V go through its own ring
+// of asynchronous copies (16-byte chunks, XOR-swizzled), scores and P V through m16n8k16 products with the
+// (at most 16) query heads of the group as rows, and running maximum and sum stay in its registers; the
+// warps meet only at the end of a unit.  Scores cost 8 KB of smem reads per 16 keys against 8 KB from HBM;
+// the products are far from any limit, so tensor memory would buy nothing here.
+#include "attention_tc.cuh"
 
 namespace sptmm {
+
+constexpr uint32_t kDecodeWarps = 4, kDecodeThreads = 32 * kDecodeWarps, kTileKeys = 16, kBlockKeys = kTileKeys * kDecodeWarps;
+constexpr uint32_t kMaxDecodeCtas = 384;     // two per SM on up to 192 SMs
+constexpr uint32_t kDecodeStages = 3;
 
 struct DecodeParams {
     const void *Q;
     void *O;
     CacheView cache;
-    const int32_t *lengths, *table, *prefix_table;
+    const int32_t *lengths, *table;
     uint64_t ldq, ldo;
-    uint32_t B, heads, group, max_pages, prefix_len;
-    float scale;
+    uint32_t B, heads, group, max_pages, row_tiles, rows;      // rows: query heads per unit, at most 16
+    uint32_t partial;                        // never store to O: the prefix's parts are still to be joined
+    float scale;                             // scale * log2(e)
+    uint2 *span;                             // [unit]: its first and last piece
+    float2 *part_ml;                         // [piece][rows]: (m in powers of two, l)
+    float *part_o;                           // [piece][rows][head_dim]
+    // the prefix's parts
+    const float2 *prefix_ml;
+    const float *prefix_o;
+    uint32_t splits;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(256) k_decode_rows(const DecodeParams p)
+__device__ __forceinline__ uint32_t own_keys(const DecodeParams &p, uint32_t b)
 {
-    const uint32_t lane = threadIdx.x & 31, c = lane * 4, D = p.cache.head_dim;
-    const uint64_t item = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const uint64_t room = (uint64_t)p.max_pages << p.cache.page_shift;
+    return (uint32_t)min(room, (uint64_t)max(p.lengths[b], 0));
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    if constexpr (__is_same(T, __half))
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 16 bytes, or zeros where `bytes` is 0
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+template <int DP> struct DecodeLayout {
+    static constexpr uint32_t row = DP * 2, tile = kTileKeys * row, stage = 2 * tile;      // K tile, V tile
+    static constexpr uint32_t smem = kDecodeWarps * kDecodeStages * stage;
+    static_assert(smem >= kDecodeWarps * 16 * DP * 4, "the warps' sums are exchanged in the rings' memory");
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kDecodeThreads)
+k_decode(const DecodeParams p)
+{
+    using L = DecodeLayout<DP>;
+    constexpr uint32_t chunks = DP / 8;      // 16-byte chunks of a row
+    extern __shared__ __align__(1024) unsigned char dyn[];
+    __shared__ uint64_t warp_sum[kDecodeWarps];
+    __shared__ uint32_t start_b;
+    __shared__ uint64_t start_w;
+    __shared__ float2 ml[kDecodeWarps][16];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
+    const uint32_t D = p.cache.head_dim, per_seq = p.cache.kv_heads * p.row_tiles;
     pdl_launch_dependents();
     pdl_wait_prior_grid();
-    if (item >= (uint64_t)p.B * p.heads) return;
-    const uint32_t b = (uint32_t)(item / p.heads), h = (uint32_t)(item % p.heads), kh = h / p.group;
-    float q[4] = {0, 0, 0, 0}, o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0;
-    if (c < D) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const T *>(p.Q) + (uint64_t)b * p.ldq + (uint64_t)h * D + c);
-        const float2 a = unpack2<T>(w.x), d = unpack2<T>(w.y);
-        q[0] = a.x * p.scale; q[1] = a.y * p.scale; q[2] = d.x * p.scale; q[3] = d.y * p.scale;
+    // ---- this CTA's run of blocks: thread t sums a contiguous range of sequences -----------------------
+    const uint32_t each = (p.B + kDecodeThreads - 1) / kDecodeThreads, b_lo = min(p.B, tid * each), b_hi = min(p.B, b_lo + each);
+    uint64_t mine = 0;
+    for (uint32_t b = b_lo; b < b_hi; b++) mine += (uint64_t)((own_keys(p, b) + kBlockKeys - 1) / kBlockKeys) * per_seq;
+    uint64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= (uint32_t)o) upto += y;
     }
-    const uint64_t room = (uint64_t)p.max_pages << p.cache.page_shift;
-    const uint32_t own = (uint32_t)min(room, (uint64_t)max(p.lengths[b], 0));
-    for (uint32_t part = 0; part < 2; part++) {
-        const int32_t *table = part ? p.table + (uint64_t)b * p.max_pages : p.prefix_table;
-        const uint32_t n = part ? own : p.prefix_len;
-        for (uint32_t j = 0; j < n; j++) {
-            const uint32_t page = (uint32_t)table[j >> p.cache.page_shift];
-            if (page >= p.cache.n_pages) continue;
-            float k[4] = {0, 0, 0, 0}, v[4] = {0, 0, 0, 0};
-            if (c < D) {
-                const uint64_t at = p.cache.at(page, kh, j & (p.cache.page_size() - 1)) + c;
-                const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const T *>(p.cache.k) + at);
-                const uint2 z = *reinterpret_cast<const uint2 *>(static_cast<const T *>(p.cache.v) + at);
-                float2 a = unpack2<T>(w.x), d = unpack2<T>(w.y);
-                k[0] = a.x; k[1] = a.y; k[2] = d.x; k[3] = d.y;
-                a = unpack2<T>(z.x); d = unpack2<T>(z.y);
-                v[0] = a.x; v[1] = a.y; v[2] = d.x; v[3] = d.y;
+    if (lane == 31) warp_sum[warp] = upto;
+    __syncthreads();
+    uint64_t total = 0, before = upto - mine;
+    for (uint32_t w = 0; w < kDecodeWarps; w++) {
+        if (w < warp) before += warp_sum[w];
+        total += warp_sum[w];
+    }
+    // no CTA between two that work may stay empty, or a unit's pieces would not be neighbours
+    const uint64_t active = min((uint64_t)gridDim.x, total);
+    if (cta >= active) return;
+    const uint64_t w0 = total * cta / active, w1 = total * (cta + 1) / active;
+    if (before <= w0 && w0 < before + mine) {
+        uint64_t at = before;
+        uint32_t b = b_lo;
+        for (;; b++) {
+            const uint64_t nb = (uint64_t)((own_keys(p, b) + kBlockKeys - 1) / kBlockKeys) * per_seq;
+            if (w0 < at + nb) break;
+            at += nb;
+        }
+        start_b = b; start_w = at;
+    }
+    __syncthreads();
+    uint32_t b = start_b;
+    uint64_t at = start_w;                   // number of the first block of sequence b
+    const uint32_t ring = smem_addr(dyn) + warp * kDecodeStages * L::stage;
+    uint64_t w = w0;
+    while (w < w1) {
+        const uint32_t len = own_keys(p, b), nb = (len + kBlockKeys - 1) / kBlockKeys;
+        if (nb == 0 || w >= at + (uint64_t)nb * per_seq) { at += (uint64_t)nb * per_seq; b++; continue; }
+        const uint32_t sub = (uint32_t)((w - at) / nb), kh = sub / p.row_tiles, rt = sub % p.row_tiles;
+        const uint32_t blk0 = (uint32_t)((w - at) % nb), blk1 = (uint32_t)min((uint64_t)nb, blk0 + (w1 - w));
+        const uint32_t unit = b * per_seq + sub, piece = unit + cta;
+        const uint32_t head0 = kh * p.group + rt * 16, rows = min(p.rows, p.group - rt * 16);
+        const int32_t *table = p.table + (uint64_t)b * p.max_pages;
+
+        // tile i of this warp: keys from ((blk0 + i) * warps + warp) * 16
+        const uint32_t tiles = blk1 - blk0;
+        auto key_of = [&](uint32_t i) { return ((blk0 + i) * kDecodeWarps + warp) * kTileKeys; };
+        auto page_of = [&](uint32_t i) -> uint32_t {
+            const uint32_t key = key_of(i);
+            return i < tiles && key < len ? (uint32_t)table[key >> p.cache.page_shift] : 0xffffffffu;
+        };
+        uint32_t page_lane = page_of(lane);          // pages of tiles page_base .. + 32, one per lane
+        uint32_t page_base = 0, page_next = page_of(32 + lane);
+        uint32_t valid_bits = 0;                     // bit s: the tile in ring slot s lies in the cache
+        auto issue = [&](uint32_t i) {
+            if (i < tiles) {
+                if (i - page_base >= 32) { page_base += 32; page_lane = page_next; page_next = page_of(page_base + 32 + lane); }
+                const uint32_t page = __shfl_sync(0xffffffffu, page_lane, i - page_base);
+                const uint32_t key0 = key_of(i), slot = i % kDecodeStages;
+                const bool good = page < p.cache.n_pages;
+                valid_bits = (valid_bits & ~(1u << slot)) | (uint32_t)good << slot;
+                const uint64_t base = good ? p.cache.at(page, kh, key0 & (p.cache.page_size() - 1)) : 0;
+                const uint32_t dst = ring + slot * L::stage;
+#pragma unroll
+                for (uint32_t x = 0; x < kTileKeys * chunks / 32; x++) {
+                    const uint32_t r = (x * 32 + lane) / chunks, c = (x * 32 + lane) % chunks;
+                    const uint32_t bytes = good && key0 + r < len && c * 8 < D ? 16 : 0;
+                    const uint64_t off = bytes ? base + r * D + c * 8 : 0;
+                    const uint32_t to = dst + r * L::row + ((c ^ (r & 7)) << 4);
+                    copy16(to, static_cast<const T *>(p.cache.k) + off, bytes);
+                    copy16(to + L::tile, static_cast<const T *>(p.cache.v) + off, bytes);
+                }
             }
-            float s = q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3];
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
 #pragma unroll
-            for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-            const float m1 = fmaxf(m, s), w0 = m1 == -INFINITY ? 1.0f : exp2f(m - m1), w1 = m1 == -INFINITY ? 0.0f : exp2f(s - m1);
-            m = m1;
-            l = l * w0 + w1;
+        for (uint32_t s = 0; s < kDecodeStages - 1; s++) issue(s);
+
+        // query rows as A fragments: rows lane / 4 and + 8, channels 2 (lane % 4) and + 8 of every sixteen
+        uint32_t qa[DP / 16][4];
+        const T *q = static_cast<const T *>(p.Q) + (uint64_t)b * p.ldq + (uint64_t)head0 * D;
 #pragma unroll
-            for (int i = 0; i < 4; i++) o[i] = o[i] * w0 + w1 * v[i];
+        for (int k = 0; k < DP / 16; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t r = lane / 4 + (e & 1) * 8, c = k * 16 + (lane & 3) * 2 + (e >> 1) * 8;
+                qa[k][e] = r < rows && c < D ? *reinterpret_cast<const uint32_t *>(q + (uint64_t)r * D + c) : 0u;
+            }
+        float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0, 0};
+#pragma unroll
+        for (int n = 0; n < DP / 8; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[n][e] = 0.0f;
+
+        for (uint32_t i = 0; i < tiles; i++) {
+            issue(i + kDecodeStages - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kDecodeStages - 1) : "memory");
+            __syncwarp();
+            const uint32_t key0 = key_of(i), slot = i % kDecodeStages, kb = ring + slot * L::stage, vb = kb + L::tile;
+            if (key0 < len && (valid_bits >> slot & 1)) {
+                float s[2][4] = {};
+#pragma unroll
+                for (int k = 0; k < DP / 16; k++) {
+                    const uint32_t r = (lane & 7) + (lane >> 4) * 8, c = k * 2 + (lane >> 3 & 1);
+                    uint32_t f[4];
+                    ldsm4(kb + r * L::row + ((c ^ (r & 7)) << 4), f);
+                    mma16816<T>(s[0], qa[k], f[0], f[1]);
+                    mma16816<T>(s[1], qa[k], f[2], f[3]);
+                }
+                const uint32_t col = key0 + (lane & 3) * 2;
+                if (key0 + kTileKeys > len) {
+#pragma unroll
+                    for (int n = 0; n < 2; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) if (col + n * 8 + (e & 1) >= len) s[n][e] = -INFINITY;
+                }
+                float mx[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    mx[h] = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)) * p.scale;
+                }
+                // scale down only when a maximum has grown by more than 2^8 (or is the first)
+                const bool grow = (mx[0] > m[0] && (m[0] == -INFINITY || mx[0] - m[0] > 8.0f)) || (mx[1] > m[1] && (m[1] == -INFINITY || mx[1] - m[1] > 8.0f));
+                if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const float m1 = fmaxf(m[h], mx[h]), f = m[h] == -INFINITY ? (m1 == -INFINITY ? 1.0f : 0.0f) : ex2(m[h] - m1);
+                        m[h] = m1; l[h] *= f;
+#pragma unroll
+                        for (int n = 0; n < DP / 8; n++) { o[n][2 * h] *= f; o[n][2 * h + 1] *= f; }
+                    }
+                }
+                uint32_t pa[4];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float base = m[h] == -INFINITY ? 0.0f : m[h];
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        const float x = ex2(fmaf(s[n][2 * h], p.scale, -base)), y = ex2(fmaf(s[n][2 * h + 1], p.scale, -base));
+                        l[h] += x + y;
+                        pa[n * 2 + h] = pack2<T>(x, y);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < DP / 16; n++) {
+                    const uint32_t r = (lane & 7) + (lane >> 3 & 1) * 8, c = n * 2 + (lane >> 4);
+                    uint32_t f[4];
+                    ldsm4_t(vb + r * L::row + ((c ^ (r & 7)) << 4), f);
+                    mma16816<T>(o[2 * n], pa, f[0], f[1]);
+                    mma16816<T>(o[2 * n + 1], pa, f[2], f[3]);
+                }
+            }
+            __syncwarp();
+        }
+        // ---- the warps' parts -> one ---------------------------------------------------------------
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            if ((lane & 3) == 0) ml[warp][lane / 4 + h * 8] = make_float2(m[h], l[h]);
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();                     // every ring is idle: its memory holds the warps' sums from here
+        float *sums = reinterpret_cast<float *>(dyn);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t r = lane / 4 + h * 8;
+            if (r < rows) {
+                float M = -INFINITY;
+                for (uint32_t x = 0; x < kDecodeWarps; x++) M = fmaxf(M, ml[x][r].x);
+                const float f = m[h] == -INFINITY ? 0.0f : ex2(m[h] - M);
+#pragma unroll
+                for (int n = 0; n < DP / 8; n++)
+                    *reinterpret_cast<float2 *>(sums + (warp * 16 + r) * DP + n * 8 + (lane & 3) * 2) = make_float2(o[n][2 * h] * f, o[n][2 * h + 1] * f);
+            }
+        }
+        __syncthreads();
+        const bool whole = blk0 == 0 && blk1 == nb && !p.partial;
+        for (uint32_t x = tid; x < rows * (D / 4); x += kDecodeThreads) {
+            const uint32_t r = x / (D / 4), c = x % (D / 4) * 4;
+            float4 v = make_float4(0, 0, 0, 0);
+            float M = -INFINITY, sum = 0;
+            for (uint32_t y = 0; y < kDecodeWarps; y++) M = fmaxf(M, ml[y][r].x);
+            for (uint32_t y = 0; y < kDecodeWarps; y++) {
+                const float4 z = *reinterpret_cast<const float4 *>(sums + (y * 16 + r) * DP + c);
+                v.x += z.x; v.y += z.y; v.z += z.z; v.w += z.w;
+                if (ml[y][r].x != -INFINITY) sum += ml[y][r].y * ex2(ml[y][r].x - M);
+                else sum += ml[y][r].y;      // zero, or not a number
+            }
+            if (whole) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                *reinterpret_cast<uint2 *>(static_cast<T *>(p.O) + (uint64_t)b * p.ldo + (uint64_t)(head0 + r) * D + c) =
+                    make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+            } else {
+                *reinterpret_cast<float4 *>(p.part_o + ((uint64_t)piece * p.rows + r) * D + c) = v;
+                if (c == 0) p.part_ml[(uint64_t)piece * p.rows + r] = make_float2(M, sum);
+            }
+        }
+        if (tid == 0) {
+            if (blk0 == 0) p.span[unit].x = whole ? 0xffffffffu : piece;
+            if (blk1 == nb) p.span[unit].y = piece;
+        }
+        __syncthreads();                     // the sums have been read: the rings may be filled again
+        w += tiles;
+    }
+}
+
+// A warp per (sequence, query head): joins the prefix's and the pieces' parts.
+template <typename T>
+__global__ void __launch_bounds__(128) k_decode_join(const DecodeParams p)
+{
+    const uint32_t lane = threadIdx.x & 31, c = lane * 4, D = p.cache.head_dim;
+    const uint64_t row = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
+    if (row >= (uint64_t)p.B * p.heads) return;
+    const uint32_t b = (uint32_t)(row / p.heads), h = (uint32_t)(row % p.heads), kh = h / p.group, g = h % p.group;
+    const uint32_t unit = (b * p.cache.kv_heads + kh) * p.row_tiles + g / 16, r = g % 16;
+    uint32_t first = 0, count = 0;
+    if (own_keys(p, b) > 0) {
+        const uint2 s = p.span[unit];
+        if (s.x == 0xffffffffu) return;      // the whole unit went straight to O
+        first = s.x; count = s.y - s.x + 1;
+    }
+    float M = -INFINITY, l = 0, o[4] = {0, 0, 0, 0};
+    const uint32_t parts = p.splits + count;
+    auto ml_of = [&](uint32_t i) { return i < p.splits ? p.prefix_ml[row * p.splits + i] : p.part_ml[(uint64_t)(first + i - p.splits) * p.rows + r]; };
+    for (uint32_t i = lane; i < parts; i += 32) M = fmaxf(M, ml_of(i).x);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+    for (uint32_t i = 0; i < parts; i++) {
+        const float2 y = ml_of(i);
+        const float f = y.x == -INFINITY ? (y.y == 0.0f ? 0.0f : 1.0f) : ex2(y.x - M);
+        l += y.y * f;
+        if (c < D && f != 0.0f) {
+            const float *src = i < p.splits ? p.prefix_o + (row * p.splits + i) * D : p.part_o + ((uint64_t)(first + i - p.splits) * p.rows + r) * D;
+            const float4 v = *reinterpret_cast<const float4 *>(src + c);
+            o[0] += v.x * f; o[1] += v.y * f; o[2] += v.z * f; o[3] += v.w * f;
         }
     }
     if (c >= D) return;
-    const float r = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     *reinterpret_cast<uint2 *>(static_cast<T *>(p.O) + (uint64_t)b * p.ldo + (uint64_t)h * D + c) =
-        make_uint2(pack2<T>(o[0] * r, o[1] * r), pack2<T>(o[2] * r, o[3] * r));
+        make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
+}
+
+// How the prefix's keys are divided: enough parts for one CTA per SM, a block of 128 keys at least.
+struct PrefixPlan { uint32_t pairs, splits, blocks_per_split; };
+static PrefixPlan plan_prefix(uint32_t B, uint32_t kv_heads, uint32_t group, uint32_t prefix_len)
+{
+    PrefixPlan pl{};
+    if (!prefix_len) return pl;
+    const uint32_t tokens = 128 / group, blocks = (prefix_len + kKeys - 1) / kKeys;
+    pl.pairs = (B + 2 * tokens - 1) / (2 * tokens);
+    const uint64_t items = (uint64_t)pl.pairs * kv_heads;
+    const uint32_t want = items >= 148 ? 1u : (uint32_t)(148 / items);
+    pl.blocks_per_split = (blocks + want - 1) / want;
+    pl.splits = (blocks + pl.blocks_per_split - 1) / pl.blocks_per_split;
+    return pl;
+}
+
+struct WorkspacePlan { uint64_t span, part_ml, part_o, prefix_ml, prefix_o, bytes; uint32_t row_tiles, rows; PrefixPlan prefix; };
+static WorkspacePlan plan_workspace(uint32_t B, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t prefix_len)
+{
+    WorkspacePlan w{};
+    const uint32_t group = heads / kv_heads;
+    w.row_tiles = (group + 15) / 16; w.rows = group < 16 ? group : 16;
+    w.prefix = plan_prefix(B, kv_heads, group, prefix_len);
+    const uint64_t units = (uint64_t)B * kv_heads * w.row_tiles, pieces = units + kMaxDecodeCtas, parts = (uint64_t)B * heads * w.prefix.splits;
+    uint64_t cur = 0;
+    auto take = [&](uint64_t bytes) { const uint64_t at = cur; cur += (bytes + 255) & ~255ull; return at; };
+    w.span = take(units * sizeof(uint2));
+    w.part_ml = take(pieces * w.rows * sizeof(float2));
+    w.part_o = take(pieces * w.rows * head_dim * sizeof(float));
+    w.prefix_ml = take(parts * sizeof(float2));
+    w.prefix_o = take(parts * head_dim * sizeof(float));
+    w.bytes = cur;
+    return w;
+}
+
+template <typename T, int DP>
+static cudaError_t launch_decode(const DecodeParams &d, const TcParams &t, const PrefixPlan &pl, const CUtensorMap *maps, uint32_t ctas, void *stream, bool pdl)
+{
+    cudaError_t e;
+    if (pl.splits) {
+        e = cudaFuncSetAttribute(k_attention_tc<T, DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<DP>::smem);
+        if (e != cudaSuccess) return e;
+        e = launch(k_attention_tc<T, DP, true>, dim3(pl.pairs * t.kv_heads * pl.splits), dim3(kTcThreads), TcLayout<DP>::smem, stream, pdl, t, maps[0], maps[1], maps[2]);
+        if (e != cudaSuccess) return e;
+        pdl = true;
+    }
+    e = cudaFuncSetAttribute(k_decode<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeLayout<DP>::smem);
+    if (e != cudaSuccess) return e;
+    e = launch(k_decode<T, DP>, dim3(ctas), dim3(kDecodeThreads), DecodeLayout<DP>::smem, stream, pdl, d);
+    if (e != cudaSuccess) return e;
+    return launch(k_decode_join<T>, dim3((uint32_t)(((uint64_t)d.B * d.heads + 3) / 4)), dim3(128), 0, stream, true, d);
 }
 
 }  // namespace sptmm
@@ -72,9 +403,10 @@ using namespace sptmm;
 
 extern "C" uint64_t sptmm_attention_decode_workspace(uint32_t B, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t prefix_len)
 {
-    if (check_heads("attention_decode_workspace", heads, kv_heads, head_dim, SPTMM_F16) != SPTMM_OK) return 0;
-    (void)prefix_len;
-    return 16 * ((uint64_t)B + 1);
+    const char *who = "attention_decode_workspace";
+    if (check_heads(who, heads, kv_heads, head_dim, SPTMM_F16) != SPTMM_OK) return 0;
+    if (B > 65536 || prefix_len > 0x7fffffffu - 128) { fail(SPTMM_ERR_INVALID, "%s: B=%u prefix_len=%u", who, B, prefix_len); return 0; }
+    return plan_workspace(B, heads, kv_heads, head_dim, prefix_len).bytes;
 }
 
 extern "C" int sptmm_attention_decode(const sptmm_decode_params *a, uint32_t flags, void *stream)
@@ -102,12 +434,47 @@ extern "C" int sptmm_attention_decode(const sptmm_decode_params *a, uint32_t fla
     const uint64_t need = sptmm_attention_decode_workspace(a->B, a->heads, a->cache->kv_heads, a->cache->head_dim, a->prefix_len);
     if (!a->workspace || a->workspace_bytes < need)
         return fail(SPTMM_ERR_INVALID, "%s: workspace of %llu bytes, %llu needed", who, (unsigned long long)(a->workspace ? a->workspace_bytes : 0), (unsigned long long)need);
-    prm.Q = a->Q; prm.O = a->O; prm.lengths = a->lengths; prm.table = a->table; prm.prefix_table = a->prefix_table;
-    prm.B = a->B; prm.heads = a->heads; prm.group = a->heads / a->cache->kv_heads; prm.max_pages = a->max_pages; prm.prefix_len = a->prefix_len;
-    prm.scale = (a->scale > 0.0f ? a->scale : 1.0f / sqrtf((float)a->cache->head_dim)) * 1.4426950408889634f;      // log2(e): the kernel works with exp2
-    const dim3 grid((uint32_t)(((uint64_t)a->B * a->heads + 7) / 8));
-    const cudaError_t e = a->cache->dtype == SPTMM_F16 ? launch(k_decode_rows<__half>, grid, dim3(256), 0, stream, flags & SPTMM_LAUNCH_PDL, prm)
-                                                       : launch(k_decode_rows<__nv_bfloat16>, grid, dim3(256), 0, stream, flags & SPTMM_LAUNCH_PDL, prm);
+    const uint32_t kv_heads = a->cache->kv_heads, D = a->cache->head_dim, group = a->heads / kv_heads, dtype = a->cache->dtype;
+    const WorkspacePlan w = plan_workspace(a->B, a->heads, kv_heads, D, a->prefix_len);
+    if ((uint64_t)a->B * kv_heads * w.row_tiles + kMaxDecodeCtas > 0x7fffffffull || (uint64_t)w.prefix.pairs * kv_heads * w.prefix.splits > 0x7fffffffull ||
+        (uint64_t)a->B * a->heads > 0x7fffffffull)
+        return fail(SPTMM_ERR_UNSUPPORTED, "%s: %u sequences of %u key heads in one call", who, a->B, kv_heads);
+    char *ws = static_cast<char *>(a->workspace);
+    prm.Q = a->Q; prm.O = a->O; prm.lengths = a->lengths; prm.table = a->table;
+    prm.B = a->B; prm.heads = a->heads; prm.group = group; prm.max_pages = a->max_pages;
+    prm.row_tiles = w.row_tiles; prm.rows = w.rows; prm.partial = a->prefix_len ? 1 : 0;
+    prm.scale = (a->scale > 0.0f ? a->scale : 1.0f / sqrtf((float)D)) * 1.4426950408889634f;      // log2(e): the kernels work with exp2
+    prm.span = reinterpret_cast<uint2 *>(ws + w.span);
+    prm.part_ml = reinterpret_cast<float2 *>(ws + w.part_ml); prm.part_o = reinterpret_cast<float *>(ws + w.part_o);
+    prm.prefix_ml = reinterpret_cast<float2 *>(ws + w.prefix_ml); prm.prefix_o = reinterpret_cast<float *>(ws + w.prefix_o);
+    prm.splits = w.prefix.splits;
+    TcParams t{};
+    CUtensorMap maps[3];
+    if (a->prefix_len) {
+        t.Q = a->Q; t.ldq = prm.ldq; t.T = a->B; t.heads = a->heads; t.kv_heads = kv_heads; t.group = group; t.head_dim = D;
+        t.tokens = 128 / group; t.scale = prm.scale;
+        t.prefix_table = a->prefix_table; t.prefix_len = a->prefix_len; t.n_pages = prm.cache.n_pages; t.page_shift = prm.cache.page_shift;
+        t.splits = w.prefix.splits; t.blocks_per_split = w.prefix.blocks_per_split;
+        t.part_o = reinterpret_cast<float *>(ws + w.prefix_o); t.part_ml = reinterpret_cast<float2 *>(ws + w.prefix_ml);
+        rc = attention_status_word(&t.status);
+        if (rc != SPTMM_OK) return rc;
+        const uint64_t dims_q[3] = {D, a->heads, a->B}, str_q[2] = {D * 2ull, prm.ldq * 2};
+        const uint64_t dims_k[4] = {D, a->cache->page_size, kv_heads, a->cache->n_pages};
+        const uint64_t str_k[3] = {D * 2ull, (uint64_t)a->cache->page_size * D * 2, prm.cache.page_stride * 2};
+        const uint32_t box_q[3] = {64, group, t.tokens}, box_k[4] = {64, a->cache->page_size, 1, 1};
+        rc = make_tensor_map(who, &maps[0], a->Q, dtype, 3, dims_q, str_q, box_q);
+        if (rc == SPTMM_OK) rc = make_tensor_map(who, &maps[1], a->cache->k, dtype, 4, dims_k, str_k, box_k);
+        if (rc == SPTMM_OK) rc = make_tensor_map(who, &maps[2], a->cache->v, dtype, 4, dims_k, str_k, box_k);
+        if (rc != SPTMM_OK) return rc;
+    }
+    int dev = 0, sms = 0;
+    SPTMM_CUDA_TRY(cudaGetDevice(&dev));
+    SPTMM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    const uint32_t ctas = 2 * (uint32_t)sms < kMaxDecodeCtas ? 2 * (uint32_t)sms : kMaxDecodeCtas;
+    const bool pdl = flags & SPTMM_LAUNCH_PDL, wide = D > 64;
+    cudaError_t e;
+    if (dtype == SPTMM_F16) e = wide ? launch_decode<__half, 128>(prm, t, w.prefix, maps, ctas, stream, pdl) : launch_decode<__half, 64>(prm, t, w.prefix, maps, ctas, stream, pdl);
+    else e = wide ? launch_decode<__nv_bfloat16, 128>(prm, t, w.prefix, maps, ctas, stream, pdl) : launch_decode<__nv_bfloat16, 64>(prm, t, w.prefix, maps, ctas, stream, pdl);
     if (e != cudaSuccess) return fail(SPTMM_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     return SPTMM_OK;
 }
