@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from typing import Optional
 
 import numpy as np
@@ -478,8 +479,25 @@ class _DecodeParams(C.Structure):
                 + [(n, C.c_uint32) for n in ("B", "heads", "max_pages", "prefix_len")] + [("scale", C.c_float)])
 
 
-def _opt(x):
-    return _ptr(x) if x is not None else None
+def _packer(cls):
+    """The bytes of a parameter structure from its fields' values in order: packing them costs a third of
+    filling the ctypes object, which counts in calls of a few microseconds."""
+    code = {C.c_void_p: "Q", C.c_uint64: "Q", C.c_uint32: "I", C.c_float: "f"}
+    fmt = "@" + "".join(code[t] for _, t in cls._fields_)
+    return struct.Struct(fmt + "%dx" % (C.sizeof(cls) - struct.calcsize(fmt))).pack
+
+
+_pack_rotate, _pack_prompt, _pack_decode = _packer(_RotateParams), _packer(_PromptParams), _packer(_DecodeParams)
+
+
+def _addr(x) -> int:
+    """As _ptr, torch tensors first; 0 for None."""
+    if x is None:
+        return 0
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        return _ptr(x)
 
 
 class KVCache:
@@ -489,6 +507,7 @@ class KVCache:
     def __init__(self, k, v, n_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: int = F16, page_stride: int = 0):
         self._keep = (k, v)
         self.struct = _KVCacheStruct(_ptr(k), _ptr(v), dtype, n_pages, page_size, kv_heads, head_dim, 0, page_stride)
+        self.address = C.addressof(self.struct)
 
 
 def rotate_heads(QKV, T: int, heads: int, kv_heads: int, head_dim: int, positions, inv_freq, Q, in_dtype: int = F32, dtype: int = F16,
@@ -498,20 +517,23 @@ def rotate_heads(QKV, T: int, heads: int, kv_heads: int, head_dim: int, position
     """Fused qkv rows -> normalised, rotated 16-bit heads in packed rows and / or cache slots
     (sptmm_rotate_heads); device buffers, but inv_freq: one float64 per rotated channel pair, host
     (None: no rotation)."""
-    f = np.ascontiguousarray(inv_freq, dtype=np.float64) if inv_freq is not None else np.empty(0)
-    p = _RotateParams(_ptr(QKV), _opt(q_norm), _opt(k_norm), f.ctypes.data if f.size else None, _opt(positions), _opt(slots),
-                      _ptr(Q), _opt(K), _opt(V), C.addressof(cache.struct) if cache is not None else None, ldqkv, ldq, ldk, ldv,
-                      T, heads, kv_heads, head_dim, in_dtype, dtype, 2 * f.size, 1 if interleaved else 0, eps)
-    check(lib.sptmm_rotate_heads(C.byref(p), flags, stream))
+    pairs, f = 0, None
+    if inv_freq is not None:
+        f = np.ascontiguousarray(inv_freq, dtype=np.float64)
+        pairs = f.size
+    p = _pack_rotate(_addr(QKV), _addr(q_norm), _addr(k_norm), f.__array_interface__["data"][0] if pairs else 0, _addr(positions),
+                     _addr(slots), _addr(Q), _addr(K), _addr(V), cache.address if cache is not None else 0, ldqkv, ldq, ldk, ldv,
+                     T, heads, kv_heads, head_dim, in_dtype, dtype, 2 * pairs, 1 if interleaved else 0, eps)
+    check(lib.sptmm_rotate_heads(p, flags, stream))
 
 
 def attention_prompt(Q, K, V, out, q_offsets, k_offsets, n_seqs: int, T: int, Tk: int, heads: int, kv_heads: int, head_dim: int,
                      dtype: int = F16, causal: bool = True, scale: float = 0.0, ldq: int = 0, ldk: int = 0, ldv: int = 0, ldo: int = 0,
                      flags: int = 0, stream: int = 0) -> None:
     """Attention over packed sequences (sptmm_attention_prompt); device buffers, scale 0 = 1 / sqrt(head_dim)."""
-    p = _PromptParams(_ptr(Q), _opt(K), _opt(V), _ptr(out), _ptr(q_offsets), _ptr(k_offsets), ldq, ldk, ldv, ldo,
-                      n_seqs, T, Tk, heads, kv_heads, head_dim, dtype, 1 if causal else 0, scale)
-    check(lib.sptmm_attention_prompt(C.byref(p), flags, stream))
+    p = _pack_prompt(_addr(Q), _addr(K), _addr(V), _addr(out), _addr(q_offsets), _addr(k_offsets), ldq, ldk, ldv, ldo,
+                     n_seqs, T, Tk, heads, kv_heads, head_dim, dtype, 1 if causal else 0, scale)
+    check(lib.sptmm_attention_prompt(p, flags, stream))
 
 
 def attention_decode_workspace(B: int, heads: int, kv_heads: int, head_dim: int, prefix_len: int = 0) -> int:
@@ -526,9 +548,9 @@ def attention_decode(Q, out, B: int, heads: int, cache: KVCache, lengths, table,
                      workspace=None, workspace_bytes: int = 0, scale: float = 0.0, ldq: int = 0, ldo: int = 0,
                      flags: int = 0, stream: int = 0) -> None:
     """One new token per sequence over a paged cache, behind an optional shared prefix (sptmm_attention_decode)."""
-    p = _DecodeParams(_ptr(Q), _ptr(out), C.addressof(cache.struct), _ptr(lengths), _opt(table), _opt(prefix_table), _opt(workspace),
-                      workspace_bytes, ldq, ldo, B, heads, max_pages, prefix_len, scale)
-    check(lib.sptmm_attention_decode(C.byref(p), flags, stream))
+    p = _pack_decode(_addr(Q), _addr(out), cache.address, _addr(lengths), _addr(table), _addr(prefix_table), _addr(workspace),
+                     workspace_bytes, ldq, ldo, B, heads, max_pages, prefix_len, scale)
+    check(lib.sptmm_attention_decode(p, flags, stream))
 
 
 def attention_status() -> int:
