@@ -43,7 +43,7 @@ struct TcParams {
     uint32_t *status;
 };
 
-constexpr uint32_t kTcThreads = 352;
+constexpr uint32_t kTcThreads = 384;        // three warpgroups: two of softmax, one of loads, products and the value check
 constexpr uint32_t kKeys = 128;              // keys per block
 
 template <int DP> struct TcLayout {
@@ -247,6 +247,9 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
     uint32_t issued = 0;                     // ring loads on their way (the loading thread's)
     const bool cut = (it.block0 + n) * kKeys > last_key;                            // the last block holds keys nobody sees
 
+    // registers: 3 x 168 at launch; a softmax thread holds 128 scores, the others next to nothing
+    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp < 8) {
         // ---- softmax: thread = row --------------------------------------------------------------
         const uint32_t tile = warp >> 2, row = tid & 127, s_addr = tmem + tile * 128 + ((warp & 3) << 21), o_addr = tmem + 256 + tile * DP + ((warp & 3) << 21);
@@ -457,7 +460,7 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                 }
             }
         }
-    } else if (!PREFIX && n > 0 && p.causal) {
+    } else if (!PREFIX && warp == 10 && n > 0 && p.causal) {
         // ---- values that some rows here see and others do not: all finite? --------------------------
         const uint32_t from = it.visible(it.first);
         uint32_t found = 0;
