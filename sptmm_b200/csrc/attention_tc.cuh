@@ -185,19 +185,19 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
     using L = TcLayout<DP>;
     constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
     extern __shared__ unsigned char dyn[];
-    __shared__ uint64_t bars[2 + 2 * L::stages + 2 + 2 + 2 + 1 + 1];
+    __shared__ uint64_t bars[2 + 2 * L::stages + 2 + 4 + 2 + 1 + 1];
     __shared__ uint32_t tmem_base, abort_flag, bad_values, item_seq, item_pair, item_ok;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t bar0 = smem_addr(bars);
     const uint32_t b_q = bar0, b_full = bar0 + 16, b_empty = b_full + 8 * L::stages, b_s = b_empty + 8 * L::stages, b_p = b_s + 16,
-                   b_o = b_p + 16, b_fix = b_o + 16, b_end = b_fix + 8;
+                   b_o = b_p + 32, b_fix = b_o + 16, b_end = b_fix + 8;
     volatile uint32_t *abort_word = &abort_flag;
     pdl_launch_dependents();
     if (warp == 8) {
         if (lane == 0) {
             mbar_init(b_q, 1); mbar_init(b_q + 8, 1);
             for (uint32_t i = 0; i < L::stages; i++) { mbar_init(b_full + 8 * i, 1); mbar_init(b_empty + 8 * i, 1); }
-            for (uint32_t t = 0; t < 2; t++) { mbar_init(b_s + 8 * t, 1); mbar_init(b_p + 8 * t, 4); mbar_init(b_o + 8 * t, 1); }
+            for (uint32_t t = 0; t < 2; t++) { mbar_init(b_s + 8 * t, 1); mbar_init(b_p + 16 * t, 4); mbar_init(b_p + 16 * t + 8, 4); mbar_init(b_o + 8 * t, 1); }
             mbar_init(b_fix, 1); mbar_init(b_end, 1);
             abort_flag = 0; bad_values = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -269,8 +269,8 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                     if (lane < per && (at << p.page_shift) < p.prefix_len) good = (uint32_t)p.prefix_table[at] < p.n_pages;
                     pages_ok = __ballot_sync(0xffffffffu, good);
                 }
-                if (!mbar_wait(b_s + 8 * tile, i & 1, abort_word)) ok = false;
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                ok = ok && mbar_wait_warp(b_s + 8 * tile, i & 1, abort_word);
+                if (!ok) break;
                 tc_fence_after();
                 uint32_t r[128];
 #pragma unroll
@@ -317,25 +317,26 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                 const float base = m == -INFINITY ? 0.0f : m * sc;
                 const uint64_t sc2 = f2_pack(sc, sc), nb2 = f2_pack(-base, -base);
                 uint64_t sum[2] = {0, 0};
-                uint32_t w[64];
 #pragma unroll
-                for (int c = 0; c < 128; c += 2) {
-                    const float2 x = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sc2, nb2));
-                    const float a = ex2(x.x), b = ex2(x.y);
-                    sum[(c >> 1) & 1] = f2_add(sum[(c >> 1) & 1], f2_pack(a, b));
-                    w[c >> 1] = pack2<T>(a, b);
+                for (int half = 0; half < 2; half++) {                               // the product starts on the first half
+                    uint32_t w[32];
+#pragma unroll
+                    for (int c = 0; c < 64; c += 2) {
+                        const float2 x = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[64 * half + c]), __uint_as_float(r[64 * half + c + 1])), sc2, nb2));
+                        const float a = ex2(x.x), b = ex2(x.y);
+                        sum[(c >> 1) & 1] = f2_add(sum[(c >> 1) & 1], f2_pack(a, b));
+                        w[c >> 1] = pack2<T>(a, b);
+                    }
+                    tmem_st32(s_addr + 32 * half, w);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(b_p + 16 * tile + 8 * half);
                 }
-                tmem_st32(s_addr, w);
-                tmem_st32(s_addr + 32, w + 32);
                 const float2 z = f2_unpack(f2_add(sum[0], sum[1]));
                 l += z.x + z.y;
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(b_p + 8 * tile);
             }
-            if (ok && !mbar_wait(b_o + 8 * tile, 0, abort_word)) ok = false;
-            ok = __all_sync(0xffffffffu, ok);
+            ok = ok && mbar_wait_warp(b_o + 8 * tile, 0, abort_word);
             tc_fence_after();
         }
         // ---- epilogue ----
@@ -410,7 +411,7 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
         // zeros over the values that nobody here sees
         if (ok && n > 0 && cut) {
             const uint32_t x = 2 * n - 1, st = x % L::stages;
-            if (mbar_wait(b_full + 8 * st, x / L::stages & 1, abort_word)) {
+            if (mbar_wait_warp(b_full + 8 * st, x / L::stages & 1, abort_word)) {
                 const uint32_t from = last_key - (it.block0 + n - 1) * kKeys;
                 for (uint32_t s = 0; s < slabs; s++)
                     for (uint32_t a = from * 128 + lane * 16; a < 16384; a += 512)
@@ -422,42 +423,56 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
         }
     } else if (warp == 9) {
         // ---- products ----------------------------------------------------------------------------
-        if (lane == 0 && n > 0) {
-            const uint32_t steps = (D + 15) / 16;
+        if (n > 0) {
+            const uint32_t steps = (D + 15) / 16, last_step = steps - 1;
             const uint32_t desc_s = mma_desc(kBf16, 128, false), desc_o = mma_desc(kBf16, steps * 16, true);
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const bool leader = elect_one();
             bool ok = true;
             auto scores = [&](uint32_t t, uint32_t x) {                              // S_t = Q_t K^T, K in ring use x
-                const uint32_t kb = ring + x % L::stages * L::tile, qb = q_smem + t * L::tile;
-                for (uint32_t k = 0; k < steps; k++) {
-                    const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-                    mma_ss(tmem + t * 128, smem_desc(qb + off, 0, 1024), smem_desc(kb + off, 0, 1024), desc_s, k > 0);
+                const uint64_t kb = smem_desc(ring + x % L::stages * L::tile, 0, 1024), qb = smem_desc(q_smem + t * L::tile, 0, 1024);
+                if (leader) {
+#pragma unroll
+                    for (uint32_t k = 0; k < DP / 16; k++) {
+                        const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+                        if (k <= last_step) mma_ss(tm + t * 128, qb + off, kb + off, desc_s, k > 0);
+                    }
+                    tc_commit(b_s + 8 * t);
                 }
-                tc_commit(b_s + 8 * t);
+                __syncwarp();
             };
-            auto full = [&](uint32_t x) { return mbar_wait(b_full + 8 * (x % L::stages), x / L::stages & 1, abort_word); };
+            auto full = [&](uint32_t x) { return mbar_wait_warp(b_full + 8 * (x % L::stages), x / L::stages & 1, abort_word); };
             ok = full(0);
             for (uint32_t t = 0; t < n_tiles && ok; t++) {
-                ok = mbar_wait(b_q + 8 * t, 0, abort_word);
+                ok = mbar_wait_warp(b_q + 8 * t, 0, abort_word);
                 if (ok) { tc_fence_after(); scores(t, 0); }
             }
-            if (ok) tc_commit(b_empty);
+            if (ok && leader) tc_commit(b_empty);
             for (uint32_t i = 0; i < n && ok; i++) {
                 const bool last = i + 1 == n;
-                ok = full(2 * i + 1) && (last || full(2 * i + 2)) && (!last || !cut || mbar_wait(b_fix, 0, abort_word));
-                const uint32_t vb = ring + (2 * i + 1) % L::stages * L::tile;
+                ok = full(2 * i + 1) && (last || full(2 * i + 2)) && (!last || !cut || mbar_wait_warp(b_fix, 0, abort_word));
+                const uint64_t vb = smem_desc(ring + (2 * i + 1) % L::stages * L::tile, 16384, 1024);
                 for (uint32_t t = 0; t < n_tiles && ok; t++) {
-                    ok = mbar_wait(b_p + 8 * t, i & 1, abort_word);
+                    for (uint32_t half = 0; half < 2 && ok; half++) {                // O_t += P_t V, sixteen keys at a time
+                        ok = mbar_wait_warp(b_p + 16 * t + 8 * half, i & 1, abort_word);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (leader) {
+#pragma unroll
+                            for (uint32_t k = 0; k < 4; k++)
+                                mma_ts(tm + 256 + t * DP, tm + t * 128 + (4 * half + k) * 8, vb + (4 * half + k) * 128, desc_o, i > 0 || half > 0 || k > 0);
+                        }
+                        __syncwarp();
+                    }
                     if (!ok) break;
-                    tc_fence_after();
-                    for (uint32_t k = 0; k < 8; k++)                                 // O_t += P_t V, sixteen keys at a time
-                        mma_ts(tmem + 256 + t * DP, tmem + t * 128 + k * 8, smem_desc(vb + k * 2048, 16384, 1024), desc_o, i > 0 || k > 0);
                     if (!last) scores(t, 2 * i + 2);
-                    else tc_commit(b_o + 8 * t);
+                    else if (leader) tc_commit(b_o + 8 * t);
                 }
-                if (ok) {
+                if (ok && leader) {
                     tc_commit(b_empty + 8 * ((2 * i + 1) % L::stages));
                     if (!last) tc_commit(b_empty + 8 * ((2 * i + 2) % L::stages));
                 }
+                __syncwarp();
             }
         }
     } else if (!PREFIX && warp == 10 && n > 0 && p.causal) {
@@ -482,8 +497,9 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
         // a wait ran out (never in a healthy run): report, then let copies and products in flight end
         if (tid == 0) atomicOr(p.status, 1u);
         uint32_t never = 0;
-        if (tid == 9 * 32 && n > 0) {
-            tc_commit(b_end);                // arrives when every product issued so far is done
+        if (warp == 9 && n > 0) {
+            __syncwarp();
+            if (elect_one()) tc_commit(b_end);       // arrives when every product issued so far is done
             mbar_wait(b_end, 0, &never);
         }
         if (tid == 8 * 32 && n > 0) {

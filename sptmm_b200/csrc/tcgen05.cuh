@@ -41,6 +41,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return false;
 }
 
+// The same by a whole warp, with one answer for all lanes (an abort may be seen by some lanes first).
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t *abort_word)
+{
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_word));
+}
+
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z)
 {
     asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -129,6 +135,15 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 {
     asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+
+// One lane of a converged warp.  The products are issued by code the whole warp walks through, with only
+// the instructions themselves under this predicate: their operands then stay in uniform registers.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t ok;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(ok));
+    return ok;
 }
 
 __device__ __forceinline__ float ex2(float x)
