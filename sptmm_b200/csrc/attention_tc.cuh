@@ -429,40 +429,47 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             const bool leader = elect_one();
             bool ok = true;
+            const uint32_t k_hi = smem_desc(0, 0, 1024) >> 32, v_hi = smem_desc(0, 16384, 1024) >> 32;
+            auto slot_lo = [&](uint32_t addr, uint32_t lead) { return (uint32_t)smem_desc(addr, lead, 1024); };
             auto scores = [&](uint32_t t, uint32_t x) {                              // S_t = Q_t K^T, K in ring use x
-                const uint64_t kb = smem_desc(ring + x % L::stages * L::tile, 0, 1024), qb = smem_desc(q_smem + t * L::tile, 0, 1024);
+                const uint32_t kb = slot_lo(ring + x % L::stages * L::tile, 0), qb = slot_lo(q_smem + t * L::tile, 0);
                 if (leader) {
 #pragma unroll
                     for (uint32_t k = 0; k < DP / 16; k++) {
                         const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-                        if (k <= last_step) mma_ss(tm + t * 128, qb + off, kb + off, desc_s, k > 0);
+                        if (k <= last_step) mma_ss(tm + t * 128, qb + off, k_hi, kb + off, k_hi, desc_s, k > 0);
                     }
                     tc_commit(b_s + 8 * t);
                 }
                 __syncwarp();
             };
             auto full = [&](uint32_t x) { return mbar_wait_warp(b_full + 8 * (x % L::stages), x / L::stages & 1, abort_word); };
+            // A wait costs a hundred cycles even when there is nothing to wait for: those for loads come
+            // right behind an issued product, while it runs.
             ok = full(0);
             for (uint32_t t = 0; t < n_tiles && ok; t++) {
                 ok = mbar_wait_warp(b_q + 8 * t, 0, abort_word);
                 if (ok) { tc_fence_after(); scores(t, 0); }
             }
             if (ok && leader) tc_commit(b_empty);
+            ok = ok && full(1);
             for (uint32_t i = 0; i < n && ok; i++) {
                 const bool last = i + 1 == n;
-                ok = full(2 * i + 1) && (last || full(2 * i + 2)) && (!last || !cut || mbar_wait_warp(b_fix, 0, abort_word));
-                const uint64_t vb = smem_desc(ring + (2 * i + 1) % L::stages * L::tile, 16384, 1024);
+                if (last && cut) ok = mbar_wait_warp(b_fix, 0, abort_word);
+                const uint32_t vb = slot_lo(ring + (2 * i + 1) % L::stages * L::tile, 16384);
                 for (uint32_t t = 0; t < n_tiles && ok; t++) {
-                    for (uint32_t half = 0; half < 2 && ok; half++) {                // O_t += P_t V, sixteen keys at a time
-                        ok = mbar_wait_warp(b_p + 16 * t + 8 * half, i & 1, abort_word);
+#pragma unroll
+                    for (uint32_t half = 0; half < 2; half++) {                      // O_t += P_t V, sixteen keys at a time
+                        ok = ok && mbar_wait_warp(b_p + 16 * t + 8 * half, i & 1, abort_word);
                         if (!ok) break;
                         tc_fence_after();
                         if (leader) {
 #pragma unroll
                             for (uint32_t k = 0; k < 4; k++)
-                                mma_ts(tm + 256 + t * DP, tm + t * 128 + (4 * half + k) * 8, vb + (4 * half + k) * 128, desc_o, i > 0 || half > 0 || k > 0);
+                                mma_ts(tm + 256 + t * DP, tm + t * 128 + (4 * half + k) * 8, vb + (4 * half + k) * 128, v_hi, desc_o, i > 0 || half > 0 || k > 0);
                         }
                         __syncwarp();
+                        if (t == 0 && half == 0 && !last) ok = full(2 * i + 2);
                     }
                     if (!ok) break;
                     if (!last) scores(t, 2 * i + 2);
@@ -473,6 +480,7 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                     if (!last) tc_commit(b_empty + 8 * ((2 * i + 2) % L::stages));
                 }
                 __syncwarp();
+                if (ok && !last) ok = full(2 * i + 3);
             }
         }
     } else if (!PREFIX && warp == 10 && n > 0 && p.causal) {
