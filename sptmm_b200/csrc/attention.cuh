@@ -86,17 +86,29 @@ inline int check_cache(const char *who, const sptmm_kv_cache *c, CacheView &v)
     return SPTMM_OK;
 }
 
-// One launch, with the programmatic-dependent-launch attribute when `pdl`.
+// One launch, with the programmatic-dependent-launch attribute when `pdl`, in clusters when `cluster` > 1.
 template <typename... P, typename... A>
-inline cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, void *stream, bool pdl, A &&...args)
+inline cudaError_t launch_clusters(uint32_t cluster, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, void *stream, bool pdl, A &&...args)
 {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = pdl ? 1 : 0;
+    cudaLaunchAttribute attr[2];
+    uint32_t n = 0;
+    if (pdl) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster; attr[n].val.clusterDim.y = 1; attr[n++].val.clusterDim.z = 1;
+    }
+    cfg.attrs = attr; cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+template <typename... P, typename... A>
+inline cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, void *stream, bool pdl, A &&...args)
+{
+    return launch_clusters(1, kernel, grid, block, smem, stream, pdl, static_cast<A &&>(args)...);
 }
 
 }  // namespace sptmm

@@ -34,10 +34,13 @@ struct TcParams {
     uint64_t ldq, ldk, ldv, ldo;
     uint32_t n_seqs, T, Tk, heads, kv_heads, group, head_dim, causal;
     uint32_t tokens;                         // tokens per tile, 128 / group
+    uint32_t cluster;                        // CTAs that may share an item's keys
+    uint32_t group_mul;                      // x * group_mul >> 16 = x / group for x < 128
     float scale;                             // scale * log2(e)
     // the shared prefix of a decode step: keys in pages, parts of the keys in different CTAs
     const int32_t *prefix_table;
-    uint32_t prefix_len, n_pages, page_shift, splits, blocks_per_split;
+    uint32_t prefix_len, n_pages, page_shift;
+    uint32_t splits;                         // clusters per item, each with an equal part of the keys
     float *part_o;                           // [token][head][split][head_dim], not divided by l
     float2 *part_ml;                         // [token][head][split]: (m in powers of two, l)
     uint32_t *status;
@@ -50,7 +53,34 @@ template <int DP> struct TcLayout {
     static constexpr uint32_t slabs = DP / 64, tile = 128 * DP * 2;
     static constexpr uint32_t stages = DP == 128 ? 5 : 8;
     static constexpr uint32_t smem = 2 * tile + stages * tile + 1024;      // 1024: room to align
+    static constexpr uint32_t out = 256 * DP * 4;                          // the ring's memory at the end: O in fp32, then (m, l) of every row
+    static_assert(out + 256 * 8 <= stages * tile, "the ring holds O and (m, l) at the end");
 };
+
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the address of `addr` in the shared memory of CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t smem_of(uint32_t addr, uint32_t rank)
+{
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr)
+{
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 
 // One row by CUDA cores: a warp, four channels per lane, keys k0 .. k0 + n one after the other.
 template <typename T>
@@ -117,6 +147,14 @@ __device__ __forceinline__ void seq_range(const TcParams &p, uint32_t s, uint32_
 __device__ __forceinline__ bool find_item(const TcParams &p, uint32_t w, uint32_t &seq, uint32_t &pair)
 {
     const uint32_t lane = threadIdx.x & 31, per = 2 * p.tokens;
+    if (p.n_seqs == 1) {
+        uint32_t q0, nq, k0, m;
+        seq_range(p, 0, q0, nq, k0, m);
+        const uint32_t n = (nq + per - 1) / per;
+        seq = 0;
+        pair = p.causal ? n - 1 - w : w;
+        return w < n;
+    }
     // items and first level of sequence s
     auto shape = [&](uint32_t s, uint32_t &n, uint32_t &low) {
         uint32_t q0, nq, k0, m;
@@ -177,7 +215,9 @@ __device__ __forceinline__ bool find_item(const TcParams &p, uint32_t w, uint32_
     return false;
 }
 
-template <typename T, int DP, bool PREFIX>
+// SPLIT: clusters share the keys of an item.  A variant of its own, because what it keeps for the end costs the
+// others registers in the softmax loop (8192 tokens: 323 us against 275).
+template <typename T, int DP, bool PREFIX, bool SPLIT>
 __global__ void __launch_bounds__(kTcThreads, 1)
 k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                const __grid_constant__ CUtensorMap map_v)
@@ -207,15 +247,16 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
         tmem_alloc(smem_addr(&tmem_base), 512);
     }
     pdl_wait_prior_grid();
+    const uint32_t rank = SPLIT ? blockIdx.x % p.cluster : 0, unit = SPLIT ? blockIdx.x / p.cluster : blockIdx.x;
     uint32_t kh, split = 0;
     if constexpr (PREFIX) {
-        split = blockIdx.x % p.splits;
-        kh = blockIdx.x / p.splits % p.kv_heads;
+        split = unit % p.splits;
+        kh = unit / p.splits % p.kv_heads;
     } else {
-        kh = blockIdx.x % p.kv_heads;
+        kh = unit % p.kv_heads;
         if (warp == 0) {
             uint32_t s = 0, pr = 0;
-            const bool ok = find_item(p, blockIdx.x / p.kv_heads, s, pr);
+            const bool ok = find_item(p, unit / p.kv_heads, s, pr);
             if (lane == 0) { item_ok = ok; item_seq = s; item_pair = pr; }
         }
     }
@@ -223,20 +264,28 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
     __syncthreads();
     tc_fence_after();
     TcItem it;
+    bool spread;                             // the CTAs of the cluster share the item's keys
     if constexpr (PREFIX) {
         it.q0 = 0; it.n_q = p.T; it.k0 = 0; it.m = p.prefix_len; it.shift = (int32_t)p.prefix_len;
-        it.first = blockIdx.x / p.splits / p.kv_heads * 2 * p.tokens;
+        it.first = unit / p.splits / p.kv_heads * 2 * p.tokens;
         it.any = true;
-        it.block0 = split * p.blocks_per_split;
-        it.blocks = min((p.prefix_len + kKeys - 1) / kKeys, it.block0 + p.blocks_per_split) - it.block0;
+        spread = SPLIT && p.cluster > 1;
+        const uint32_t all = (p.prefix_len + kKeys - 1) / kKeys, parts = p.splits * p.cluster, part = split * p.cluster + rank;
+        it.block0 = (uint32_t)((uint64_t)all * part / parts);
+        it.blocks = (uint32_t)((uint64_t)all * (part + 1) / parts) - it.block0;
     } else {
         it.any = item_ok;
         seq_range(p, it.any ? item_seq : 0, it.q0, it.n_q, it.k0, it.m);
         it.shift = p.causal ? (int32_t)it.m - (int32_t)it.n_q : 0x40000000;
         it.first = (it.any ? item_pair : 0) * 2 * p.tokens;
-        it.block0 = 0;
-        it.blocks = it.any ? (it.visible(min(it.n_q, it.first + 2 * p.tokens) - 1) + kKeys - 1) / kKeys : 0;
+        const uint32_t all = it.any ? (it.visible(min(it.n_q, it.first + 2 * p.tokens) - 1) + kKeys - 1) / kKeys : 0;
+        // two blocks each are the least that pays for the exchange at the end; else the first CTA alone
+        spread = SPLIT && all >= 2 * p.cluster;
+        it.any = it.any && (spread || rank == 0);
+        it.block0 = spread ? all * rank / p.cluster : 0;
+        it.blocks = spread ? all * (rank + 1) / p.cluster - it.block0 : it.any ? all : 0;
     }
+    const bool joined = PREFIX || spread;    // O leaves through the rows' parts in shared memory
     const uint32_t n_here = it.any ? min(it.n_q - it.first, 2 * p.tokens) : 0;      // queries of this CTA
     const uint32_t n_tiles = n_here > p.tokens ? 2 : 1;
     const uint32_t last_key = it.any ? it.visible(it.first + n_here - 1) : 0;       // keys nobody here sees start at this one
@@ -253,7 +302,7 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
     if (warp < 8) {
         // ---- softmax: thread = row --------------------------------------------------------------
         const uint32_t tile = warp >> 2, row = tid & 127, s_addr = tmem + tile * 128 + ((warp & 3) << 21), o_addr = tmem + 256 + tile * DP + ((warp & 3) << 21);
-        const uint32_t tok = tile * p.tokens + row / p.group, head = kh * p.group + row % p.group;      // row / group < tokens for rows in use
+        const uint32_t tok = tile * p.tokens + row / p.group;      // row / group < tokens for rows in use
         const bool mine = row < p.tokens * p.group && tok < n_here;
         const uint32_t vis = mine ? it.visible(it.first + tok) : it.m;         // rows not in use are never stored: no mask for their sake
         float m = -INFINITY, l = 0.0f;       // m in units of the raw score
@@ -337,44 +386,119 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                 l += z.x + z.y;
             }
             ok = ok && mbar_wait_warp(b_o + 8 * tile, 0, abort_word);
+            if (joined) ok = ok && (n_tiles == 1 || mbar_wait_warp(b_o + 8 * (tile ^ 1), 0, abort_word));
             tc_fence_after();
         }
-        // ---- epilogue ----
-        if (ok && tile < n_tiles) {
-            if constexpr (PREFIX) {
-                const uint64_t at = ((uint64_t)(it.first + tok) * p.heads + head) * p.splits + split;
-                if (mine) p.part_ml[at] = make_float2(m == -INFINITY ? -INFINITY : m * sc, l);
+        // ---- out ----
+        if (joined) {
+            if (ok && tile < n_tiles && n > 0) {
+                // every product is done: the ring's memory takes O (16-byte chunks swizzled by row) and (m, l)
+                const uint32_t to = ring + (tile * 128 + row) * DP * 4;
+                asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(ring + L::out + (tile * 128 + row) * 8), "f"(m == -INFINITY ? -INFINITY : m * sc), "f"(l) : "memory");
                 for (uint32_t c = 0; c < D; c += 32) {
                     uint32_t o[32];
                     tmem_ld32(o_addr + c, o);
                     tmem_wait_ld();
                     pin32(o);
-                    if (mine)
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            if (c + e < D) *reinterpret_cast<uint4 *>(p.part_o + at * D + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (uint32_t e = 0; e < 8; e++)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (((c >> 2) + (e ^ (row & 7))) << 4)), "r"(o[4 * e]), "r"(o[4 * e + 1]),
+                                     "r"(o[4 * e + 2]), "r"(o[4 * e + 3]) : "memory");
                 }
-            } else {
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                T *out = static_cast<T *>(p.O) + (uint64_t)(it.q0 + it.first + tok) * p.ldo + (uint64_t)head * D;
-                for (uint32_t c = 0; c < D; c += 32) {
-                    uint32_t o[32] = {};
-                    if (n > 0) {
-                        tmem_ld32(o_addr + c, o);
-                        tmem_wait_ld();
-                        pin32(o);
+            }
+            // the CTAs of the cluster share the rows and read one another's parts, four rows of a warp at a time
+            // (half a warp to a row up to 64 channels)
+            if (spread) cluster_sync();
+            else asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (ok) {
+                constexpr uint32_t kLanes = DP / 4, kRows = 32 / kLanes, kBatch = 4;
+                const uint32_t c = lane % kLanes * 4, ranks = spread ? p.cluster : 1, here = n_here * p.group, step = 8 * kRows * ranks;
+                for (uint32_t x0 = (spread ? rank * 8 * kRows : 0) + warp * kRows + lane / kLanes; x0 < here; x0 += kBatch * step) {
+                    float M[kBatch], l[kBatch], f[kBatch][8];
+                    float4 o[kBatch];
+                    uint32_t R[kBatch];
+#pragma unroll
+                    for (uint32_t b = 0; b < kBatch; b++) {
+                        const uint32_t x = min(x0 + b * step, here - 1), i = x / p.group;
+                        R[b] = i / p.tokens * 128 + i % p.tokens * p.group + x % p.group;
+                        M[b] = -INFINITY; l[b] = 0; o[b] = make_float4(0, 0, 0, 0);
                     }
-                    if (mine)
+                    float2 y[kBatch][8];
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8)
-                            if (c + e < D) {
-                                uint32_t y[4];
+                    for (uint32_t s = 0; s < 8; s++)
+                        if (s < ranks)
 #pragma unroll
-                                for (int x = 0; x < 4; x++)
-                                    y[x] = vis == 0 ? 0u : pack2<T>(__uint_as_float(o[e + 2 * x]) * inv, __uint_as_float(o[e + 2 * x + 1]) * inv);
-                                *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(y[0], y[1], y[2], y[3]);
-                            }
+                            for (uint32_t b = 0; b < kBatch; b++) y[b][s] = ld_cluster2(smem_of(ring + L::out + R[b] * 8, spread ? s : rank));
+#pragma unroll
+                    for (uint32_t b = 0; b < kBatch; b++) {
+#pragma unroll
+                        for (uint32_t s = 0; s < 8; s++) if (s < ranks) M[b] = fmaxf(M[b], y[b][s].x);
+#pragma unroll
+                        for (uint32_t s = 0; s < 8; s++)
+                            if (s < ranks) { f[b][s] = y[b][s].x == -INFINITY ? (y[b][s].y == 0.0f ? 0.0f : 1.0f) : ex2(y[b][s].x - M[b]); l[b] += y[b][s].y * f[b][s]; }
+                    }
+#pragma unroll
+                    for (uint32_t s = 0; s < 8; s++)
+                        if (s < ranks) {
+                            float4 v[kBatch];
+#pragma unroll
+                            for (uint32_t b = 0; b < kBatch; b++) v[b] = ld_cluster4(smem_of(ring + R[b] * DP * 4 + (((c >> 2) ^ (R[b] & 7)) << 4), spread ? s : rank));
+#pragma unroll
+                            for (uint32_t b = 0; b < kBatch; b++)
+                                if (f[b][s] != 0.0f) { o[b].x += v[b].x * f[b][s]; o[b].y += v[b].y * f[b][s]; o[b].z += v[b].z * f[b][s]; o[b].w += v[b].w * f[b][s]; }
+                        }
+#pragma unroll
+                    for (uint32_t b = 0; b < kBatch; b++) {
+                        const uint32_t x = x0 + b * step, i = x / p.group, head = kh * p.group + x % p.group;
+                        if (x >= here || c >= D) continue;
+                        if constexpr (PREFIX) {
+                            const uint64_t at = ((uint64_t)(it.first + i) * p.heads + head) * p.splits + split;
+                            if (c == 0) p.part_ml[at] = make_float2(M[b], l[b]);
+                            *reinterpret_cast<float4 *>(p.part_o + at * D + c) = o[b];
+                        } else {
+                            const float inv = l[b] == 0.0f ? 0.0f : 1.0f / l[b];
+                            *reinterpret_cast<uint2 *>(static_cast<T *>(p.O) + (uint64_t)(it.q0 + it.first + i) * p.ldo + (uint64_t)head * D + c) =
+                                make_uint2(pack2<T>(o[b].x * inv, o[b].y * inv), pack2<T>(o[b].z * inv, o[b].w * inv));
+                        }
+                    }
                 }
+            }
+        } else if (!PREFIX && ok && tile < n_tiles) {
+            // The warp's rows through the memory of its own rows of Q (their products are done), so that lanes
+            // store neighbouring chunks of a row; a thread storing its own row touches 32 lines per instruction.
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;                           // no visible key, or none above -infinity: zeros
+            const uint32_t buf = q_smem + tile * L::tile + (warp & 3) * 32 * 128;    // rows of 128 bytes, 64 channels to a slab
+#pragma unroll
+            for (uint32_t c = 0; c < DP; c += 32) {
+                if (c >= D) break;
+                uint32_t o[32] = {};
+                if (n > 0) {
+                    tmem_ld32(o_addr + c, o);
+                    tmem_wait_ld();
+                    pin32(o);
+                }
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        y[x] = vis == 0 ? 0u : pack2<T>(__uint_as_float(o[8 * e + 2 * x]) * inv, __uint_as_float(o[8 * e + 2 * x + 1]) * inv);
+                    const uint32_t chunk = (c % 64) / 8 + e;
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(buf + c / 64 * 16384 + lane * 128 + ((chunk ^ (lane & 7)) << 4)), "r"(y[0]), "r"(y[1]),
+                                 "r"(y[2]), "r"(y[3]) : "memory");
+                }
+            }
+            __syncwarp();
+            constexpr uint32_t kChunks = DP / 8, kRows = 32 / kChunks;               // lanes per row, rows per pass
+            const uint32_t chunk = lane % kChunks;
+#pragma unroll 4
+            for (uint32_t r0 = 0; r0 < 32; r0 += kRows) {
+                const uint32_t r = r0 + lane / kChunks, R = (warp & 3) * 32 + r, q = R * p.group_mul >> 16, i = tile * p.tokens + q;
+                uint4 y;
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                             : "r"(buf + chunk / 8 * 16384 + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) : "memory");
+                if (R < p.tokens * p.group && i < n_here && chunk * 8 < D)
+                    *reinterpret_cast<uint4 *>(static_cast<T *>(p.O) + (uint64_t)(it.q0 + it.first + i) * p.ldo + (uint64_t)(kh * p.group + R - q * p.group) * D + chunk * 8) = y;
             }
         }
     } else if (warp == 8) {
@@ -483,9 +607,9 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                 if (ok && !last) ok = full(2 * i + 3);
             }
         }
-    } else if (!PREFIX && warp == 10 && n > 0 && p.causal) {
+    } else if (!PREFIX && warp == 10 && it.any && p.causal) {
         // ---- values that some rows here see and others do not: all finite? --------------------------
-        const uint32_t from = it.visible(it.first);
+        const uint32_t from = it.visible(it.first);                                  // (every CTA of a cluster looks, and finds the same)
         uint32_t found = 0;
         const uint32_t per = D / 8;                                                  // 16-byte words per row
         for (uint32_t x = lane; x < (last_key - from) * per; x += 32) {
@@ -500,6 +624,7 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
         if (__any_sync(0xffffffffu, found) && lane == 0) bad_values = 1;
     }
     __syncwarp();
+    if (warp >= 8 && spread) cluster_sync();         // the one the softmax warps pass before they join
     __syncthreads();
     if (abort_flag) {
         // a wait ran out (never in a healthy run): report, then let copies and products in flight end
@@ -515,7 +640,10 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
             for (uint32_t x = issued > L::stages ? issued - L::stages : 0; x < issued; x++) mbar_wait(b_full + 8 * (x % L::stages), x / L::stages & 1, &never);
         }
         __syncthreads();
-    } else if (!PREFIX && bad_values) {
+    }
+    if (spread) cluster_sync();              // nobody leaves while its memory is read
+    if (!PREFIX && bad_values && !abort_flag && rank == 0 && it.any) {
+        __syncthreads();                     // over the rows just written
         for (uint32_t x = warp; x < n_here * p.group; x += kTcThreads / 32) {
             const uint32_t i = it.first + x / p.group;
             attend_row<T>(p, it.q0 + i, kh * p.group + x % p.group, kh, it.k0, it.visible(i));

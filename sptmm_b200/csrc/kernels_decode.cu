@@ -345,8 +345,10 @@ __global__ void __launch_bounds__(128) k_decode_join(const DecodeParams p)
         make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
 }
 
-// How the prefix's keys are divided: enough parts for one CTA per SM, a block of 128 keys at least.
-struct PrefixPlan { uint32_t pairs, splits, blocks_per_split; };
+// How the prefix's keys are divided: one CTA per SM, a block of 128 keys at least, CTAs in clusters that join
+// their parts on chip.  `splits` clusters per item leave as many parts to k_decode_join.  A cluster of four
+// or eight needs that many free SMs of one GPC, so it is counted on 128 of the 148 SMs.
+struct PrefixPlan { uint32_t pairs, splits, cluster; };
 static PrefixPlan plan_prefix(uint32_t B, uint32_t kv_heads, uint32_t group, uint32_t prefix_len)
 {
     PrefixPlan pl{};
@@ -354,9 +356,9 @@ static PrefixPlan plan_prefix(uint32_t B, uint32_t kv_heads, uint32_t group, uin
     const uint32_t tokens = 128 / group, blocks = (prefix_len + kKeys - 1) / kKeys;
     pl.pairs = (B + 2 * tokens - 1) / (2 * tokens);
     const uint64_t items = (uint64_t)pl.pairs * kv_heads;
-    const uint32_t want = items >= 148 ? 1u : (uint32_t)(148 / items);
-    pl.blocks_per_split = (blocks + want - 1) / want;
-    pl.splits = (blocks + pl.blocks_per_split - 1) / pl.blocks_per_split;
+    const uint32_t want = items >= 128 ? 1u : (uint32_t)(128 / items), parts = want < blocks ? want : blocks;
+    pl.cluster = parts >= 8 ? 8 : parts >= 4 ? 4 : parts >= 2 ? 2 : 1;
+    pl.splits = parts / pl.cluster;
     return pl;
 }
 
@@ -384,9 +386,9 @@ static cudaError_t launch_decode(const DecodeParams &d, const TcParams &t, const
 {
     cudaError_t e;
     if (pl.splits) {
-        e = cudaFuncSetAttribute(k_attention_tc<T, DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<DP>::smem);
+        e = cudaFuncSetAttribute(k_attention_tc<T, DP, true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<DP>::smem);
         if (e != cudaSuccess) return e;
-        e = launch(k_attention_tc<T, DP, true>, dim3(pl.pairs * t.kv_heads * pl.splits), dim3(kTcThreads), TcLayout<DP>::smem, stream, pdl, t, maps[0], maps[1], maps[2]);
+        e = launch_clusters(pl.cluster, k_attention_tc<T, DP, true, true>, dim3(pl.pairs * t.kv_heads * pl.splits * pl.cluster), dim3(kTcThreads), TcLayout<DP>::smem, stream, pdl, t, maps[0], maps[1], maps[2]);
         if (e != cudaSuccess) return e;
         pdl = true;
     }
@@ -436,7 +438,7 @@ extern "C" int sptmm_attention_decode(const sptmm_decode_params *a, uint32_t fla
         return fail(SPTMM_ERR_INVALID, "%s: workspace of %llu bytes, %llu needed", who, (unsigned long long)(a->workspace ? a->workspace_bytes : 0), (unsigned long long)need);
     const uint32_t kv_heads = a->cache->kv_heads, D = a->cache->head_dim, group = a->heads / kv_heads, dtype = a->cache->dtype;
     const WorkspacePlan w = plan_workspace(a->B, a->heads, kv_heads, D, a->prefix_len);
-    if ((uint64_t)a->B * kv_heads * w.row_tiles + kMaxDecodeCtas > 0x7fffffffull || (uint64_t)w.prefix.pairs * kv_heads * w.prefix.splits > 0x7fffffffull ||
+    if ((uint64_t)a->B * kv_heads * w.row_tiles + kMaxDecodeCtas > 0x7fffffffull || (uint64_t)w.prefix.pairs * kv_heads * w.prefix.splits > 0x7fffffffull / 8 ||
         (uint64_t)a->B * a->heads > 0x7fffffffull)
         return fail(SPTMM_ERR_UNSUPPORTED, "%s: %u sequences of %u key heads in one call", who, a->B, kv_heads);
     char *ws = static_cast<char *>(a->workspace);
@@ -452,9 +454,9 @@ extern "C" int sptmm_attention_decode(const sptmm_decode_params *a, uint32_t fla
     CUtensorMap maps[3];
     if (a->prefix_len) {
         t.Q = a->Q; t.ldq = prm.ldq; t.T = a->B; t.heads = a->heads; t.kv_heads = kv_heads; t.group = group; t.head_dim = D;
-        t.tokens = 128 / group; t.scale = prm.scale;
+        t.tokens = 128 / group; t.group_mul = 65535 / group + 1; t.scale = prm.scale;
         t.prefix_table = a->prefix_table; t.prefix_len = a->prefix_len; t.n_pages = prm.cache.n_pages; t.page_shift = prm.cache.page_shift;
-        t.splits = w.prefix.splits; t.blocks_per_split = w.prefix.blocks_per_split;
+        t.splits = w.prefix.splits; t.cluster = w.prefix.cluster;
         t.part_o = reinterpret_cast<float *>(ws + w.prefix_o); t.part_ml = reinterpret_cast<float2 *>(ws + w.prefix_ml);
         rc = attention_status_word(&t.status);
         if (rc != SPTMM_OK) return rc;

@@ -41,12 +41,19 @@ int make_tensor_map(const char *who, CUtensorMap *map, const void *base, uint32_
     return SPTMM_OK;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool SPLIT>
 static cudaError_t launch_prompt(const TcParams &prm, uint32_t grid, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, void *stream, bool pdl)
 {
-    const cudaError_t e = cudaFuncSetAttribute(k_attention_tc<T, DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<DP>::smem);
+    const cudaError_t e = cudaFuncSetAttribute(k_attention_tc<T, DP, false, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<DP>::smem);
     if (e != cudaSuccess) return e;
-    return launch(k_attention_tc<T, DP, false>, dim3(grid), dim3(kTcThreads), TcLayout<DP>::smem, stream, pdl, prm, q, k, v);
+    return launch_clusters(prm.cluster, k_attention_tc<T, DP, false, SPLIT>, dim3(grid), dim3(kTcThreads), TcLayout<DP>::smem, stream, pdl, prm, q, k, v);
+}
+
+template <typename T>
+static cudaError_t launch_prompt(const TcParams &prm, uint32_t grid, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, void *stream, bool pdl)
+{
+    if (prm.head_dim > 64) return prm.cluster > 1 ? launch_prompt<T, 128, true>(prm, grid, q, k, v, stream, pdl) : launch_prompt<T, 128, false>(prm, grid, q, k, v, stream, pdl);
+    return prm.cluster > 1 ? launch_prompt<T, 64, true>(prm, grid, q, k, v, stream, pdl) : launch_prompt<T, 64, false>(prm, grid, q, k, v, stream, pdl);
 }
 
 }  // namespace sptmm
@@ -78,11 +85,19 @@ extern "C" int sptmm_attention_prompt(const sptmm_prompt_params *a, uint32_t fla
     prm.Q = a->Q; prm.K = a->K; prm.V = a->V; prm.O = a->O; prm.q_off = a->q_offsets; prm.k_off = a->k_offsets;
     prm.n_seqs = a->n_seqs; prm.T = a->T; prm.Tk = a->Tk; prm.heads = a->heads; prm.kv_heads = a->kv_heads; prm.group = a->heads / a->kv_heads;
     prm.head_dim = a->head_dim; prm.causal = a->causal ? 1 : 0;
-    prm.tokens = 128 / prm.group;
+    prm.tokens = 128 / prm.group; prm.group_mul = 65535 / prm.group + 1;
     prm.scale = (a->scale > 0.0f ? a->scale : 1.0f / sqrtf((float)a->head_dim)) * 1.4426950408889634f;     // log2(e): the kernel works with exp2
     // pairs of tiles: every sequence may end with a part of one
-    const uint64_t items = (uint64_t)a->T / (2 * prm.tokens) + (a->n_seqs < a->T ? a->n_seqs : a->T);
-    if (items * a->kv_heads > 0x7fffffffull) return fail(SPTMM_ERR_UNSUPPORTED, "%s: %u rows of %u key heads in one call", who, a->T, a->kv_heads);
+    const uint64_t per = 2 * prm.tokens, seqs = a->n_seqs < a->T ? a->n_seqs : a->T, items = ((uint64_t)a->T + seqs * (per - 1)) / per;
+    if (items * a->kv_heads > 0x7fffffffull / 8) return fail(SPTMM_ERR_UNSUPPORTED, "%s: %u rows of %u key heads in one call", who, a->T, a->kv_heads);
+    // Few items leave SMs idle: then up to eight CTAs, as many as there is an SM for, share an item's keys
+    // (if it has two blocks of keys for each; see the kernel).  512 queries over 8192 keys, 40 items: 126 us by
+    // 40 CTAs, 63 us by as many clusters of three.
+    int dev = 0, sms = 0;
+    SPTMM_CUDA_TRY(cudaGetDevice(&dev));
+    SPTMM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    const uint64_t room = (uint64_t)sms / (items * a->kv_heads);
+    prm.cluster = room > 8 ? 8 : room < 1 ? 1 : (uint32_t)room;
     rc = attention_status_word(&prm.status);
     if (rc != SPTMM_OK) return rc;
     const uint64_t D = a->head_dim, es = 2;
@@ -94,11 +109,9 @@ extern "C" int sptmm_attention_prompt(const sptmm_prompt_params *a, uint32_t fla
     if (rc == SPTMM_OK) rc = make_tensor_map(who, &mk, a->Tk ? a->K : a->Q, a->dtype, 3, dims_k, str_k, box_k);     // no keys: never read
     if (rc == SPTMM_OK) rc = make_tensor_map(who, &mv, a->Tk ? a->V : a->Q, a->dtype, 3, dims_k, str_v, box_k);
     if (rc != SPTMM_OK) return rc;
-    const uint32_t grid = (uint32_t)(items * a->kv_heads);
-    const bool pdl = flags & SPTMM_LAUNCH_PDL, wide = a->head_dim > 64;
-    cudaError_t e;
-    if (a->dtype == SPTMM_F16) e = wide ? launch_prompt<__half, 128>(prm, grid, mq, mk, mv, stream, pdl) : launch_prompt<__half, 64>(prm, grid, mq, mk, mv, stream, pdl);
-    else e = wide ? launch_prompt<__nv_bfloat16, 128>(prm, grid, mq, mk, mv, stream, pdl) : launch_prompt<__nv_bfloat16, 64>(prm, grid, mq, mk, mv, stream, pdl);
+    const uint32_t grid = (uint32_t)(items * a->kv_heads) * prm.cluster;
+    const bool pdl = flags & SPTMM_LAUNCH_PDL;
+    const cudaError_t e = a->dtype == SPTMM_F16 ? launch_prompt<__half>(prm, grid, mq, mk, mv, stream, pdl) : launch_prompt<__nv_bfloat16>(prm, grid, mq, mk, mv, stream, pdl);
     if (e != cudaSuccess) return fail(SPTMM_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     return SPTMM_OK;
 }
