@@ -77,8 +77,36 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t b
 
 template <int DP> struct DecodeLayout {
     static constexpr uint32_t row = DP * 2, tile = kTileKeys * row, stage = 2 * tile;      // K tile, V tile
-    static constexpr uint32_t smem = kDecodeWarps * kDecodeStages * stage;
-    static_assert(smem >= kDecodeWarps * 16 * DP * 4, "the warps' sums are exchanged in the rings' memory");
+    static constexpr uint32_t ring = kDecodeWarps * kDecodeStages * stage;
+    static constexpr uint32_t smem = ring + kDecodeWarps * 8 * DP * 4;                      // and eight rows of every warp's sums
+};
+
+// A run of blocks of one unit that a CTA takes on.
+struct Piece {
+    uint32_t b, kh, rt, unit, len, blk0, blk1, blocks;       // blocks: of the whole unit; blk0 .. blk1: this piece
+};
+
+// The CTA's way through its run [w, w1) of the units laid end to end.  A unit counts kUnitCost blocks more than
+// it has, the time its first loads and its end take, so that a CTA with many short units gets fewer blocks.
+constexpr uint32_t kUnitCost = 2;
+struct Walk {
+    uint64_t w, w1, at;                      // at: where sequence b begins
+    uint32_t b;
+    __device__ __forceinline__ bool next(const DecodeParams &p, uint32_t per_seq, Piece &x)
+    {
+        while (w < w1) {
+            const uint32_t len = own_keys(p, b), nb = (len + kBlockKeys - 1) / kBlockKeys, cost = nb + kUnitCost;
+            if (nb == 0 || w >= at + (uint64_t)cost * per_seq) { at += nb ? (uint64_t)cost * per_seq : 0; b++; continue; }
+            const uint32_t sub = (uint32_t)((w - at) / cost), v0 = (uint32_t)(w - at - (uint64_t)sub * cost), v1 = (uint32_t)min((uint64_t)cost, v0 + (w1 - w));
+            w += v1 - v0;
+            x.blk0 = v0 > kUnitCost ? v0 - kUnitCost : 0; x.blk1 = v1 > kUnitCost ? v1 - kUnitCost : 0;
+            if (x.blk0 == x.blk1) continue;  // only a part of the cost, none of the blocks
+            x.b = b; x.kh = sub / p.row_tiles; x.rt = sub % p.row_tiles; x.unit = b * per_seq + sub; x.len = len; x.blocks = nb;
+            return true;
+        }
+        x.blk0 = x.blk1 = 0;
+        return false;
+    }
 };
 
 template <typename T, int DP>
@@ -96,10 +124,14 @@ k_decode(const DecodeParams p)
     const uint32_t D = p.cache.head_dim, per_seq = p.cache.kv_heads * p.row_tiles;
     pdl_launch_dependents();
     pdl_wait_prior_grid();
-    // ---- this CTA's run of blocks: thread t sums a contiguous range of sequences -----------------------
+    // ---- this CTA's run: thread t sums a contiguous range of sequences ---------------------------------
+    auto cost_of = [&](uint32_t b) -> uint64_t {
+        const uint32_t nb = (own_keys(p, b) + kBlockKeys - 1) / kBlockKeys;
+        return nb ? (uint64_t)(nb + kUnitCost) * per_seq : 0;
+    };
     const uint32_t each = (p.B + kDecodeThreads - 1) / kDecodeThreads, b_lo = min(p.B, tid * each), b_hi = min(p.B, b_lo + each);
     uint64_t mine = 0;
-    for (uint32_t b = b_lo; b < b_hi; b++) mine += (uint64_t)((own_keys(p, b) + kBlockKeys - 1) / kBlockKeys) * per_seq;
+    for (uint32_t b = b_lo; b < b_hi; b++) mine += cost_of(b);
     uint64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -116,68 +148,70 @@ k_decode(const DecodeParams p)
     // no CTA between two that work may stay empty, or a unit's pieces would not be neighbours
     const uint64_t active = min((uint64_t)gridDim.x, total);
     if (cta >= active) return;
-    const uint64_t w0 = total * cta / active, w1 = total * (cta + 1) / active;
-    if (before <= w0 && w0 < before + mine) {
+    Walk walk;
+    walk.w = total * cta / active; walk.w1 = total * (cta + 1) / active;
+    if (before <= walk.w && walk.w < before + mine) {
         uint64_t at = before;
         uint32_t b = b_lo;
         for (;; b++) {
-            const uint64_t nb = (uint64_t)((own_keys(p, b) + kBlockKeys - 1) / kBlockKeys) * per_seq;
-            if (w0 < at + nb) break;
-            at += nb;
+            const uint64_t c = cost_of(b);
+            if (walk.w < at + c) break;
+            at += c;
         }
         start_b = b; start_w = at;
     }
     __syncthreads();
-    uint32_t b = start_b;
-    uint64_t at = start_w;                   // number of the first block of sequence b
-    const uint32_t ring = smem_addr(dyn) + warp * kDecodeStages * L::stage;
-    uint64_t w = w0;
-    while (w < w1) {
-        const uint32_t len = own_keys(p, b), nb = (len + kBlockKeys - 1) / kBlockKeys;
-        if (nb == 0 || w >= at + (uint64_t)nb * per_seq) { at += (uint64_t)nb * per_seq; b++; continue; }
-        const uint32_t sub = (uint32_t)((w - at) / nb), kh = sub / p.row_tiles, rt = sub % p.row_tiles;
-        const uint32_t blk0 = (uint32_t)((w - at) % nb), blk1 = (uint32_t)min((uint64_t)nb, blk0 + (w1 - w));
-        const uint32_t unit = b * per_seq + sub, piece = unit + cta;
-        const uint32_t head0 = kh * p.group + rt * 16, rows = min(p.rows, p.group - rt * 16);
-        const int32_t *table = p.table + (uint64_t)b * p.max_pages;
+    walk.b = start_b; walk.at = start_w;
 
-        // tile i of this warp: keys from ((blk0 + i) * warps + warp) * 16
-        const uint32_t tiles = blk1 - blk0;
-        auto key_of = [&](uint32_t i) { return ((blk0 + i) * kDecodeWarps + warp) * kTileKeys; };
-        auto page_of = [&](uint32_t i) -> uint32_t {
-            const uint32_t key = key_of(i);
-            return i < tiles && key < len ? (uint32_t)table[key >> p.cache.page_shift] : 0xffffffffu;
-        };
-        uint32_t page_lane = page_of(lane);          // pages of tiles page_base .. + 32, one per lane
-        uint32_t page_base = 0, page_next = page_of(32 + lane);
-        uint32_t valid_bits = 0;                     // bit s: the tile in ring slot s lies in the cache
-        auto issue = [&](uint32_t i) {
-            if (i < tiles) {
-                if (i - page_base >= 32) { page_base += 32; page_lane = page_next; page_next = page_of(page_base + 32 + lane); }
-                const uint32_t page = __shfl_sync(0xffffffffu, page_lane, i - page_base);
-                const uint32_t key0 = key_of(i), slot = i % kDecodeStages;
-                const bool good = page < p.cache.n_pages;
-                valid_bits = (valid_bits & ~(1u << slot)) | (uint32_t)good << slot;
-                const uint64_t base = good ? p.cache.at(page, kh, key0 & (p.cache.page_size() - 1)) : 0;
-                const uint32_t dst = ring + slot * L::stage;
+    Piece cur, nxt, iss;                     // worked on, after it, being requested (one of the two)
+    if (!walk.next(p, per_seq, cur)) return;
+    const uint32_t ring = smem_addr(dyn) + warp * kDecodeStages * L::stage;
+    float *sums = reinterpret_cast<float *>(dyn + L::ring);
+    // tile i of a piece, for this warp: keys from ((blk0 + i) * warps + warp) * 16
+    auto key_of = [&](const Piece &x, uint32_t i) { return ((x.blk0 + i) * kDecodeWarps + warp) * kTileKeys; };
+    auto page_of = [&](const Piece &x, uint32_t i) -> uint32_t {
+        const uint32_t key = key_of(x, i);
+        return i < x.blk1 - x.blk0 && key < x.len ? (uint32_t)p.table[(uint64_t)x.b * p.max_pages + (key >> p.cache.page_shift)] : 0xffffffffu;
+    };
+    uint32_t ii = 0, page_lane = page_of(cur, lane), page_next = page_of(cur, 32 + lane);      // pages of tiles ii & ~31 .. + 32 of `iss`, one per lane; the 32 after
+    iss = cur;
+    walk.next(p, per_seq, nxt);
+    uint32_t nxt_page = page_of(nxt, lane);
+    bool on_next = false;                    // iss is nxt
+    uint32_t ahead = 0, slot_in = 0, slot_out = 0, valid_bits = 0;      // tiles requested and not used; bit s: the tile in ring slot s lies in the cache
+    auto request = [&]() {                   // fills the ring's free slots, into the next piece if need be
+        while (ahead < kDecodeStages) {
+            if (ii == iss.blk1 - iss.blk0) {
+                if (on_next || nxt.blk0 == nxt.blk1) return;
+                iss = nxt; on_next = true; ii = 0;
+                page_lane = nxt_page; page_next = page_of(iss, 32 + lane);
+            }
+            const uint32_t page = __shfl_sync(0xffffffffu, page_lane, ii & 31);
+            const uint32_t key0 = key_of(iss, ii);
+            const bool good = page < p.cache.n_pages;
+            valid_bits = (valid_bits & ~(1u << slot_in)) | (uint32_t)good << slot_in;
+            const uint64_t base = good ? p.cache.at(page, iss.kh, key0 & (p.cache.page_size() - 1)) : 0;
+            const uint32_t dst = ring + slot_in * L::stage;
 #pragma unroll
-                for (uint32_t x = 0; x < kTileKeys * chunks / 32; x++) {
-                    const uint32_t r = (x * 32 + lane) / chunks, c = (x * 32 + lane) % chunks;
-                    const uint32_t bytes = good && key0 + r < len && c * 8 < D ? 16 : 0;
-                    const uint64_t off = bytes ? base + r * D + c * 8 : 0;
-                    const uint32_t to = dst + r * L::row + ((c ^ (r & 7)) << 4);
-                    copy16(to, static_cast<const T *>(p.cache.k) + off, bytes);
-                    copy16(to + L::tile, static_cast<const T *>(p.cache.v) + off, bytes);
-                }
+            for (uint32_t x = 0; x < kTileKeys * chunks / 32; x++) {
+                const uint32_t r = (x * 32 + lane) / chunks, c = (x * 32 + lane) % chunks;
+                const uint32_t bytes = good && key0 + r < iss.len && c * 8 < D ? 16 : 0;
+                const uint64_t off = bytes ? base + r * D + c * 8 : 0;
+                const uint32_t to = dst + r * L::row + ((c ^ (r & 7)) << 4);
+                copy16(to, static_cast<const T *>(p.cache.k) + off, bytes);
+                copy16(to + L::tile, static_cast<const T *>(p.cache.v) + off, bytes);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-#pragma unroll
-        for (uint32_t s = 0; s < kDecodeStages - 1; s++) issue(s);
-
-        // query rows as A fragments: rows lane / 4 and + 8, channels 2 (lane % 4) and + 8 of every sixteen
-        uint32_t qa[DP / 16][4];
-        const T *q = static_cast<const T *>(p.Q) + (uint64_t)b * p.ldq + (uint64_t)head0 * D;
+            slot_in = slot_in + 1 == kDecodeStages ? 0 : slot_in + 1;
+            ahead++; ii++;
+            if ((ii & 31) == 0) { page_lane = page_next; page_next = page_of(iss, ii + 32 + lane); }
+        }
+    };
+    request();
+    uint32_t qa[DP / 16][4];                 // query rows as A fragments: rows lane / 4 and + 8, channels 2 (lane % 4) and + 8 of every sixteen
+    auto load_q = [&](const Piece &x) {
+        const uint32_t rows = min(p.rows, p.group - x.rt * 16);
+        const T *q = static_cast<const T *>(p.Q) + (uint64_t)x.b * p.ldq + (uint64_t)(x.kh * p.group + x.rt * 16) * D;
 #pragma unroll
         for (int k = 0; k < DP / 16; k++)
 #pragma unroll
@@ -185,18 +219,24 @@ k_decode(const DecodeParams p)
                 const uint32_t r = lane / 4 + (e & 1) * 8, c = k * 16 + (lane & 3) * 2 + (e >> 1) * 8;
                 qa[k][e] = r < rows && c < D ? *reinterpret_cast<const uint32_t *>(q + (uint64_t)r * D + c) : 0u;
             }
+    };
+    load_q(cur);
+    for (;;) {
         float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0, 0};
 #pragma unroll
         for (int n = 0; n < DP / 8; n++)
 #pragma unroll
             for (int e = 0; e < 4; e++) o[n][e] = 0.0f;
-
+        const uint32_t tiles = cur.blk1 - cur.blk0, len = cur.len;
         for (uint32_t i = 0; i < tiles; i++) {
-            issue(i + kDecodeStages - 1);
-            asm volatile("cp.async.wait_group %0;" ::"n"(kDecodeStages - 1) : "memory");
+            request();
+            static_assert(kDecodeStages == 3, "the waits below count three slots");
+            if (ahead == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+            else if (ahead == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+            else asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncwarp();
-            const uint32_t key0 = key_of(i), slot = i % kDecodeStages, kb = ring + slot * L::stage, vb = kb + L::tile;
-            if (key0 < len && (valid_bits >> slot & 1)) {
+            const uint32_t key0 = key_of(cur, i), kb = ring + slot_out * L::stage, vb = kb + L::tile;
+            if (key0 < len && (valid_bits >> slot_out & 1)) {
                 float s[2][4] = {};
 #pragma unroll
                 for (int k = 0; k < DP / 16; k++) {
@@ -251,98 +291,136 @@ k_decode(const DecodeParams p)
                     mma16816<T>(o[2 * n + 1], pa, f[2], f[3]);
                 }
             }
-            __syncwarp();
+            __syncwarp();                    // the slot may be filled again
+            ahead--;
+            slot_out = slot_out + 1 == kDecodeStages ? 0 : slot_out + 1;
         }
-        // ---- the warps' parts -> one ---------------------------------------------------------------
+        // ---- on to the next piece: its loads and queries travel while this one's parts are joined ----
+        const Piece done = cur;
+        const bool more = nxt.blk0 != nxt.blk1;
+        if (more) {
+            if (!on_next) { iss = nxt; ii = 0; page_lane = nxt_page; page_next = page_of(iss, 32 + lane); }
+            on_next = false;
+            cur = nxt;
+            walk.next(p, per_seq, nxt);
+            nxt_page = page_of(nxt, lane);
+            request();
+            load_q(cur);
+        }
+        // ---- the warps' parts -> one, eight rows at a time -------------------------------------------
+        const uint32_t head0 = done.kh * p.group + done.rt * 16, rows = min(p.rows, p.group - done.rt * 16), piece = done.unit + cta;
+        const bool whole = done.blk0 == 0 && done.blk1 == done.blocks && !p.partial;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            if ((lane & 3) == 0) ml[warp][lane / 4 + h * 8] = make_float2(m[h], l[h]);
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        __syncthreads();                     // every ring is idle: its memory holds the warps' sums from here
-        float *sums = reinterpret_cast<float *>(dyn);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const uint32_t r = lane / 4 + h * 8;
-            if (r < rows) {
-                float M = -INFINITY;
-                for (uint32_t x = 0; x < kDecodeWarps; x++) M = fmaxf(M, ml[x][r].x);
-                const float f = m[h] == -INFINITY ? 0.0f : ex2(m[h] - M);
+            if (h * 8 >= (int)rows) break;
+            __syncthreads();                 // what was joined before has been read
+            const uint32_t r = lane / 4;
+            if ((lane & 3) == 0) ml[warp][r] = make_float2(m[h], l[h]);
+            if (r + h * 8 < rows)
 #pragma unroll
                 for (int n = 0; n < DP / 8; n++)
-                    *reinterpret_cast<float2 *>(sums + (warp * 16 + r) * DP + n * 8 + (lane & 3) * 2) = make_float2(o[n][2 * h] * f, o[n][2 * h + 1] * f);
-            }
-        }
-        __syncthreads();
-        const bool whole = blk0 == 0 && blk1 == nb && !p.partial;
-        for (uint32_t x = tid; x < rows * (D / 4); x += kDecodeThreads) {
-            const uint32_t r = x / (D / 4), c = x % (D / 4) * 4;
-            float4 v = make_float4(0, 0, 0, 0);
-            float M = -INFINITY, sum = 0;
-            for (uint32_t y = 0; y < kDecodeWarps; y++) M = fmaxf(M, ml[y][r].x);
-            for (uint32_t y = 0; y < kDecodeWarps; y++) {
-                const float4 z = *reinterpret_cast<const float4 *>(sums + (y * 16 + r) * DP + c);
-                v.x += z.x; v.y += z.y; v.z += z.z; v.w += z.w;
-                if (ml[y][r].x != -INFINITY) sum += ml[y][r].y * ex2(ml[y][r].x - M);
-                else sum += ml[y][r].y;      // zero, or not a number
-            }
-            if (whole) {
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                *reinterpret_cast<uint2 *>(static_cast<T *>(p.O) + (uint64_t)b * p.ldo + (uint64_t)(head0 + r) * D + c) =
-                    make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
-            } else {
-                *reinterpret_cast<float4 *>(p.part_o + ((uint64_t)piece * p.rows + r) * D + c) = v;
-                if (c == 0) p.part_ml[(uint64_t)piece * p.rows + r] = make_float2(M, sum);
+                    *reinterpret_cast<float2 *>(sums + (warp * 8 + r) * DP + n * 8 + (lane & 3) * 2) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+            __syncthreads();
+            const uint32_t here = min(8u, rows - h * 8);
+            for (uint32_t x = tid; x < here * (D / 4); x += kDecodeThreads) {
+                const uint32_t q = x / (D / 4), c = x % (D / 4) * 4, row = q + h * 8;
+                float4 v = make_float4(0, 0, 0, 0);
+                float M = -INFINITY, sum = 0;
+#pragma unroll
+                for (uint32_t y = 0; y < kDecodeWarps; y++) M = fmaxf(M, ml[y][q].x);
+#pragma unroll
+                for (uint32_t y = 0; y < kDecodeWarps; y++) {
+                    const float2 part = ml[y][q];
+                    const float f = part.x == -INFINITY ? (part.y == 0.0f ? 0.0f : 1.0f) : ex2(part.x - M);      // l of 0 without a key, else not a number
+                    const float4 z = *reinterpret_cast<const float4 *>(sums + (y * 8 + q) * DP + c);
+                    sum += part.y * f;
+                    v.x += z.x * f; v.y += z.y * f; v.z += z.z * f; v.w += z.w * f;
+                }
+                if (whole) {
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    *reinterpret_cast<uint2 *>(static_cast<T *>(p.O) + (uint64_t)done.b * p.ldo + (uint64_t)(head0 + row) * D + c) =
+                        make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+                } else {
+                    *reinterpret_cast<float4 *>(p.part_o + ((uint64_t)piece * p.rows + row) * D + c) = v;
+                    if (c == 0) p.part_ml[(uint64_t)piece * p.rows + row] = make_float2(M, sum);
+                }
             }
         }
         if (tid == 0) {
-            if (blk0 == 0) p.span[unit].x = whole ? 0xffffffffu : piece;
-            if (blk1 == nb) p.span[unit].y = piece;
+            if (done.blk0 == 0) p.span[done.unit].x = whole ? 0xffffffffu : piece;
+            if (done.blk1 == done.blocks) p.span[done.unit].y = piece;
         }
-        __syncthreads();                     // the sums have been read: the rings may be filled again
-        w += tiles;
+        if (!more) return;
     }
 }
 
-// A warp per (sequence, query head): joins the prefix's and the pieces' parts.
+// A CTA per (sequence, query head): joins the prefix's and the pieces' parts, a fourth of them per warp, all
+// loads of a warp on their way together.
 template <typename T>
 __global__ void __launch_bounds__(128) k_decode_join(const DecodeParams p)
 {
-    const uint32_t lane = threadIdx.x & 31, c = lane * 4, D = p.cache.head_dim;
-    const uint64_t row = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    __shared__ float2 ml[4];
+    __shared__ float4 sums[4][32];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane * 4, D = p.cache.head_dim;
+    const uint32_t b = blockIdx.x / p.heads, h = blockIdx.x % p.heads, kh = h / p.group, g = h % p.group;
+    const uint32_t unit = (b * p.cache.kv_heads + kh) * p.row_tiles + g / 16, r = g % 16;
+    const uint64_t row = blockIdx.x;
     pdl_launch_dependents();
     pdl_wait_prior_grid();
-    if (row >= (uint64_t)p.B * p.heads) return;
-    const uint32_t b = (uint32_t)(row / p.heads), h = (uint32_t)(row % p.heads), kh = h / p.group, g = h % p.group;
-    const uint32_t unit = (b * p.cache.kv_heads + kh) * p.row_tiles + g / 16, r = g % 16;
     uint32_t first = 0, count = 0;
+    const uint2 span = p.span[unit];         // not written where there are no keys: looked at below
     if (own_keys(p, b) > 0) {
-        const uint2 s = p.span[unit];
-        if (s.x == 0xffffffffu) return;      // the whole unit went straight to O
-        first = s.x; count = s.y - s.x + 1;
+        if (span.x == 0xffffffffu) return;   // the whole unit went straight to O
+        first = span.x; count = span.y - span.x + 1;
     }
-    float M = -INFINITY, l = 0, o[4] = {0, 0, 0, 0};
-    const uint32_t parts = p.splits + count;
-    auto ml_of = [&](uint32_t i) { return i < p.splits ? p.prefix_ml[row * p.splits + i] : p.part_ml[(uint64_t)(first + i - p.splits) * p.rows + r]; };
-    for (uint32_t i = lane; i < parts; i += 32) M = fmaxf(M, ml_of(i).x);
+    const uint32_t parts = p.splits + count, each = (parts + 3) / 4, i0 = min(parts, warp * each), i1 = min(parts, i0 + each);
+    float M = -INFINITY, l = 0;
+    float4 o = make_float4(0, 0, 0, 0);
+    for (uint32_t i = i0; i < i1; i += 8) {
+        float2 y[8];
+        float4 v[8];
 #pragma unroll
-    for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-    for (uint32_t i = 0; i < parts; i++) {
-        const float2 y = ml_of(i);
-        const float f = y.x == -INFINITY ? (y.y == 0.0f ? 0.0f : 1.0f) : ex2(y.x - M);
-        l += y.y * f;
-        if (c < D && f != 0.0f) {
-            const float *src = i < p.splits ? p.prefix_o + (row * p.splits + i) * D : p.part_o + ((uint64_t)(first + i - p.splits) * p.rows + r) * D;
-            const float4 v = *reinterpret_cast<const float4 *>(src + c);
-            o[0] += v.x * f; o[1] += v.y * f; o[2] += v.z * f; o[3] += v.w * f;
+        for (uint32_t k = 0; k < 8; k++) {
+            y[k] = make_float2(-INFINITY, 0.0f); v[k] = make_float4(0, 0, 0, 0);
+            if (i + k < i1) {
+                const uint32_t part = i + k;
+                const uint64_t at = part < p.splits ? row * p.splits + part : (uint64_t)(first + part - p.splits) * p.rows + r;
+                y[k] = part < p.splits ? p.prefix_ml[at] : p.part_ml[at];
+                if (c < D) v[k] = *reinterpret_cast<const float4 *>((part < p.splits ? p.prefix_o : p.part_o) + at * D + c);
+            }
+        }
+        float m1 = M;
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++) m1 = fmaxf(m1, y[k].x);
+        const float f0 = M == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : ex2(M - m1);
+        M = m1; l *= f0; o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++) {
+            const float f = y[k].x == -INFINITY ? (y[k].y == 0.0f ? 0.0f : 1.0f) : ex2(y[k].x - M);
+            l += y[k].y * f;
+            if (f != 0.0f) { o.x += v[k].x * f; o.y += v[k].y * f; o.z += v[k].z * f; o.w += v[k].w * f; }
         }
     }
-    if (c >= D) return;
+    if (lane == 0) ml[warp] = make_float2(M, l);
+    sums[warp][lane] = o;
+    __syncthreads();
+    if (warp || c >= D) return;
+    M = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+    l = 0; o = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) {
+        const float f = ml[k].x == -INFINITY ? (ml[k].y == 0.0f ? 0.0f : 1.0f) : ex2(ml[k].x - M);
+        const float4 v = sums[k][lane];
+        l += ml[k].y * f;
+        o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    *reinterpret_cast<uint2 *>(static_cast<T *>(p.O) + (uint64_t)b * p.ldo + (uint64_t)h * D + c) =
-        make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
+    *reinterpret_cast<uint2 *>(static_cast<T *>(p.O) + (uint64_t)b * p.ldo + (uint64_t)h * D + c) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
 }
 
 // How the prefix's keys are divided: one CTA per SM, a block of 128 keys at least, CTAs in clusters that join
@@ -396,7 +474,7 @@ static cudaError_t launch_decode(const DecodeParams &d, const TcParams &t, const
     if (e != cudaSuccess) return e;
     e = launch(k_decode<T, DP>, dim3(ctas), dim3(kDecodeThreads), DecodeLayout<DP>::smem, stream, pdl, d);
     if (e != cudaSuccess) return e;
-    return launch(k_decode_join<T>, dim3((uint32_t)(((uint64_t)d.B * d.heads + 3) / 4)), dim3(128), 0, stream, true, d);
+    return launch(k_decode_join<T>, dim3(d.B * d.heads), dim3(128), 0, stream, true, d);
 }
 
 }  // namespace sptmm
