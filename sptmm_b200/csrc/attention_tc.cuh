@@ -232,7 +232,7 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
     const uint32_t b_q = bar0, b_full = bar0 + 16, b_empty = b_full + 8 * L::stages, b_s = b_empty + 8 * L::stages, b_p = b_s + 16,
                    b_o = b_p + 32, b_fix = b_o + 16, b_end = b_fix + 8;
     volatile uint32_t *abort_word = &abort_flag;
-    pdl_launch_dependents();
+    if (!PREFIX) pdl_launch_dependents();
     if (warp == 8) {
         if (lane == 0) {
             mbar_init(b_q, 1); mbar_init(b_q + 8, 1);
@@ -247,6 +247,9 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
         tmem_alloc(smem_addr(&tmem_base), 512);
     }
     pdl_wait_prior_grid();
+    // The next kernel (k_decode) reads nothing this one writes: let it start as soon as what came before has
+    // ended, that is from here on, and it need not wait for this one.
+    if (PREFIX) pdl_launch_dependents();
     const uint32_t rank = SPLIT ? blockIdx.x % p.cluster : 0, unit = SPLIT ? blockIdx.x / p.cluster : blockIdx.x;
     uint32_t kh, split = 0;
     if constexpr (PREFIX) {
@@ -505,30 +508,41 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
         // ---- loads -------------------------------------------------------------------------------
         bool ok = true;
         const uint32_t group = p.group;
-        if (lane == 0 && n > 0) {
+        if (lane == 0 && n > 0)
             for (uint32_t t = 0; t < n_tiles; t++) {
                 mbar_expect(b_q + 8 * t, slabs * p.tokens * group * 128);
                 for (uint32_t s = 0; s < slabs; s++)
                     tma_load_3d(q_smem + t * L::tile + s * 16384, &map_q, b_q + 8 * t, s * 64, kh * group, it.q0 + it.first + t * p.tokens);
             }
+        if constexpr (PREFIX) {
+            // A block is up to eight pages of up to two slabs, a box each: lane s * 8 + g loads slab s of page g,
+            // whose number it looked up a block ahead.
+            const uint32_t size = 1u << p.page_shift, g = lane & 7, s = lane >> 3;
+            auto page_of = [&](uint32_t i) -> int32_t {                             // outside the cache: a page that reads as zeros
+                const uint32_t key = (it.block0 + i) * kKeys + g * size;
+                if (i >= n || g * size >= kKeys || key >= p.prefix_len) return (int32_t)p.n_pages;
+                const uint32_t page = (uint32_t)p.prefix_table[key >> p.page_shift];
+                return page < p.n_pages ? (int32_t)page : (int32_t)p.n_pages;
+            };
+            int32_t page = page_of(0), next = page_of(1);
+            for (uint32_t x = 0; x < 2 * n && ok; x++) {                            // K0 V0 K1 V1 ...
+                const uint32_t st = x % L::stages, use = x / L::stages, i = x >> 1;
+                if (use > 0 && !mbar_wait_warp(b_empty + 8 * st, (use - 1) & 1, abort_word)) { ok = false; break; }
+                issued = x + 1;
+                const uint32_t bar = b_full + 8 * st, keys = min(kKeys, p.prefix_len - (it.block0 + i) * kKeys), pages = (keys + size - 1) >> p.page_shift;
+                if (lane == 0) mbar_expect(bar, slabs * pages * size * 128);
+                __syncwarp();
+                if (g < pages && s < slabs) tma_load_4d(ring + st * L::tile + s * 16384 + g * size * 128, x & 1 ? &map_v : &map_k, bar, s * 64, 0, kh, page);
+                if (x & 1) { page = next; next = page_of(i + 2); }
+            }
+        } else if (lane == 0) {
             for (uint32_t x = 0; x < 2 * n && ok; x++) {                            // K0 V0 K1 V1 ...
                 const uint32_t st = x % L::stages, use = x / L::stages, i = x >> 1;
                 if (use > 0 && !mbar_wait(b_empty + 8 * st, (use - 1) & 1, abort_word)) { ok = false; break; }
                 issued = x + 1;
-                const CUtensorMap *map = x & 1 ? &map_v : &map_k;
                 const uint32_t dst = ring + st * L::tile, bar = b_full + 8 * st, j0 = (it.block0 + i) * kKeys;
-                if constexpr (PREFIX) {
-                    const uint32_t size = 1u << p.page_shift, keys = min(kKeys, p.prefix_len - j0), pages = (keys + size - 1) >> p.page_shift;
-                    mbar_expect(bar, slabs * pages * size * 128);
-                    for (uint32_t g = 0; g < pages; g++) {
-                        const uint32_t page = (uint32_t)p.prefix_table[(j0 >> p.page_shift) + g];
-                        const int32_t at = page < p.n_pages ? (int32_t)page : (int32_t)p.n_pages;       // outside the cache: reads as zeros
-                        for (uint32_t s = 0; s < slabs; s++) tma_load_4d(dst + s * 16384 + g * size * 128, map, bar, s * 64, 0, kh, at);
-                    }
-                } else {
-                    mbar_expect(bar, slabs * 16384);
-                    for (uint32_t s = 0; s < slabs; s++) tma_load_3d(dst + s * 16384, map, bar, s * 64, kh, it.k0 + j0);
-                }
+                mbar_expect(bar, slabs * 16384);
+                for (uint32_t s = 0; s < slabs; s++) tma_load_3d(dst + s * 16384, x & 1 ? &map_v : &map_k, bar, s * 64, kh, it.k0 + j0);
             }
         }
         ok = __shfl_sync(0xffffffffu, (uint32_t)ok, 0);

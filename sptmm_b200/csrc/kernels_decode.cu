@@ -123,7 +123,11 @@ k_decode(const DecodeParams p)
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
     const uint32_t D = p.cache.head_dim, per_seq = p.cache.kv_heads * p.row_tiles;
     pdl_launch_dependents();
-    pdl_wait_prior_grid();
+    // Behind the prefix's kernel this one starts when all that came before has ended (that kernel lets it go only
+    // then) and reads nothing of the prefix's: it runs beside it, and waits at its own end so that the joining
+    // kernel, which waits for this one, finds both done.
+    auto end = [&]() { if (p.partial) pdl_wait_prior_grid(); };
+    if (!p.partial) pdl_wait_prior_grid();
     // ---- this CTA's run: thread t sums a contiguous range of sequences ---------------------------------
     auto cost_of = [&](uint32_t b) -> uint64_t {
         const uint32_t nb = (own_keys(p, b) + kBlockKeys - 1) / kBlockKeys;
@@ -147,7 +151,7 @@ k_decode(const DecodeParams p)
     }
     // no CTA between two that work may stay empty, or a unit's pieces would not be neighbours
     const uint64_t active = min((uint64_t)gridDim.x, total);
-    if (cta >= active) return;
+    if (cta >= active) { end(); return; }
     Walk walk;
     walk.w = total * cta / active; walk.w1 = total * (cta + 1) / active;
     if (before <= walk.w && walk.w < before + mine) {
@@ -164,7 +168,7 @@ k_decode(const DecodeParams p)
     walk.b = start_b; walk.at = start_w;
 
     Piece cur, nxt, iss;                     // worked on, after it, being requested (one of the two)
-    if (!walk.next(p, per_seq, cur)) return;
+    if (!walk.next(p, per_seq, cur)) { end(); return; }
     const uint32_t ring = smem_addr(dyn) + warp * kDecodeStages * L::stage;
     float *sums = reinterpret_cast<float *>(dyn + L::ring);
     // tile i of a piece, for this warp: keys from ((blk0 + i) * warps + warp) * 16
@@ -355,8 +359,9 @@ k_decode(const DecodeParams p)
             if (done.blk0 == 0) p.span[done.unit].x = whole ? 0xffffffffu : piece;
             if (done.blk1 == done.blocks) p.span[done.unit].y = piece;
         }
-        if (!more) return;
+        if (!more) break;
     }
+    end();
 }
 
 // A CTA per (sequence, query head): joins the prefix's and the pieces' parts, a fourth of them per warp, all
