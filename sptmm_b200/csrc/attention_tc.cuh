@@ -35,12 +35,12 @@ struct TcParams {
     uint32_t n_seqs, T, Tk, heads, kv_heads, group, head_dim, causal;
     uint32_t tokens;                         // tokens per tile, 128 / group
     uint32_t cluster;                        // CTAs that may share an item's keys
-    uint32_t group_mul;                      // x * group_mul >> 16 = x / group for x < 128
+    uint32_t group_mul;                      // x * group_mul >> 16 = x / group for x < 256
     float scale;                             // scale * log2(e)
     // the shared prefix of a decode step: keys in pages, parts of the keys in different CTAs
     const int32_t *prefix_table;
     uint32_t prefix_len, n_pages, page_shift;
-    uint32_t splits;                         // clusters per item, each with an equal part of the keys
+    uint32_t splits;                         // CTAs per item, each with an equal part of the keys
     float *part_o;                           // [token][head][split][head_dim], not divided by l
     float2 *part_ml;                         // [token][head][split]: (m in powers of two, l)
     uint32_t *status;
@@ -217,7 +217,7 @@ __device__ __forceinline__ bool find_item(const TcParams &p, uint32_t w, uint32_
 
 // SPLIT: clusters share the keys of an item.  A variant of its own, because what it keeps for the end costs the
 // others registers in the softmax loop (8192 tokens: 323 us against 275).
-template <typename T, int DP, bool PREFIX, bool SPLIT>
+template <typename T, int DP, bool PREFIX, bool SPLIT = false>
 __global__ void __launch_bounds__(kTcThreads, 1)
 k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                const __grid_constant__ CUtensorMap map_v)
@@ -272,10 +272,10 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
         it.q0 = 0; it.n_q = p.T; it.k0 = 0; it.m = p.prefix_len; it.shift = (int32_t)p.prefix_len;
         it.first = unit / p.splits / p.kv_heads * 2 * p.tokens;
         it.any = true;
-        spread = SPLIT && p.cluster > 1;
-        const uint32_t all = (p.prefix_len + kKeys - 1) / kKeys, parts = p.splits * p.cluster, part = split * p.cluster + rank;
-        it.block0 = (uint32_t)((uint64_t)all * part / parts);
-        it.blocks = (uint32_t)((uint64_t)all * (part + 1) / parts) - it.block0;
+        spread = false;
+        const uint32_t all = (p.prefix_len + kKeys - 1) / kKeys;
+        it.block0 = (uint32_t)((uint64_t)all * split / p.splits);
+        it.blocks = (uint32_t)((uint64_t)all * (split + 1) / p.splits) - it.block0;
     } else {
         it.any = item_ok;
         seq_range(p, it.any ? item_seq : 0, it.q0, it.n_q, it.k0, it.m);
@@ -288,7 +288,6 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
         it.block0 = spread ? all * rank / p.cluster : 0;
         it.blocks = spread ? all * (rank + 1) / p.cluster - it.block0 : it.any ? all : 0;
     }
-    const bool joined = PREFIX || spread;    // O leaves through the rows' parts in shared memory
     const uint32_t n_here = it.any ? min(it.n_q - it.first, 2 * p.tokens) : 0;      // queries of this CTA
     const uint32_t n_tiles = n_here > p.tokens ? 2 : 1;
     const uint32_t last_key = it.any ? it.visible(it.first + n_here - 1) : 0;       // keys nobody here sees start at this one
@@ -389,11 +388,11 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                 l += z.x + z.y;
             }
             ok = ok && mbar_wait_warp(b_o + 8 * tile, 0, abort_word);
-            if (joined) ok = ok && (n_tiles == 1 || mbar_wait_warp(b_o + 8 * (tile ^ 1), 0, abort_word));
+            if (SPLIT && spread) ok = ok && (n_tiles == 1 || mbar_wait_warp(b_o + 8 * (tile ^ 1), 0, abort_word));
             tc_fence_after();
         }
         // ---- out ----
-        if (joined) {
+        if (SPLIT && spread) {
             if (ok && tile < n_tiles && n > 0) {
                 // every product is done: the ring's memory takes O (16-byte chunks swizzled by row) and (m, l)
                 const uint32_t to = ring + (tile * 128 + row) * DP * 4;
@@ -409,62 +408,90 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                                      "r"(o[4 * e + 2]), "r"(o[4 * e + 3]) : "memory");
                 }
             }
-            // the CTAs of the cluster share the rows and read one another's parts, four rows of a warp at a time
-            // (half a warp to a row up to 64 channels)
-            if (spread) cluster_sync();
-            else asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (ok) {
-                constexpr uint32_t kLanes = DP / 4, kRows = 32 / kLanes, kBatch = 4;
-                const uint32_t c = lane % kLanes * 4, ranks = spread ? p.cluster : 1, here = n_here * p.group, step = 8 * kRows * ranks;
-                for (uint32_t x0 = (spread ? rank * 8 * kRows : 0) + warp * kRows + lane / kLanes; x0 < here; x0 += kBatch * step) {
-                    float M[kBatch], l[kBatch], f[kBatch][8];
-                    float4 o[kBatch];
-                    uint32_t R[kBatch];
+            // the CTAs of the cluster share the rows: first every row's weights, a thread per row, then the rows,
+            // eight of a warp at a time (half a warp to a row up to 64 channels)
+            cluster_sync();
+            constexpr uint32_t kLanes = DP / 4, kRows = 32 / kLanes, kBatch = 8;
+            const uint32_t ranks = p.cluster, used = p.tokens * p.group, here = n_here * p.group, weights = q_smem;      // weights: Q is done with; 8 factors and 1 / l per row
+            auto place = [&](uint32_t x) { return x + (x >= used ? 128 - used : 0); };       // row x of those in use, counted over both tiles
+            const uint32_t share = (here + ranks - 1) / ranks, x_lo = rank * share, x_hi = min(here, x_lo + share);
+            if (x_lo + tid < x_hi) {
+                float2 y[8];
+                float M = -INFINITY, sum = 0.0f;
+#pragma unroll
+                for (uint32_t s = 0; s < 8; s++) {
+                    y[s] = make_float2(-INFINITY, 0.0f);
+                    if (s < ranks) y[s] = ld_cluster2(smem_of(ring + L::out + place(x_lo + tid) * 8, s));
+                }
+#pragma unroll
+                for (uint32_t s = 0; s < 8; s++) M = fmaxf(M, y[s].x);
+#pragma unroll
+                for (uint32_t s = 0; s < 8; s++) {
+                    const float f = y[s].x == -INFINITY ? (y[s].y == 0.0f ? 0.0f : 1.0f) : ex2(y[s].x - M);
+                    sum += y[s].y * f;
+                    y[s].x = f;
+                }
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+                for (uint32_t s = 0; s < 8; s++) asm volatile("st.shared.f32 [%0], %1;" ::"r"(weights + (tid * 8 + s) * 4), "f"(y[s].x == 0.0f ? 0.0f : y[s].x * inv) : "memory");
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const uint32_t c = lane % kLanes * 4;
+            for (uint32_t x0 = x_lo + warp * kRows + lane / kLanes; x0 - lane / kLanes < x_hi && ok; x0 += kBatch * 8 * kRows) {
+                float4 o[kBatch];
+#pragma unroll
+                for (uint32_t b = 0; b < kBatch; b++) o[b] = make_float4(0, 0, 0, 0);
+                for (uint32_t s = 0; s < ranks; s++) {
+                    const uint32_t from = smem_of(ring, s);
+                    float4 v[kBatch];
 #pragma unroll
                     for (uint32_t b = 0; b < kBatch; b++) {
-                        const uint32_t x = min(x0 + b * step, here - 1), i = x / p.group;
-                        R[b] = i / p.tokens * 128 + i % p.tokens * p.group + x % p.group;
-                        M[b] = -INFINITY; l[b] = 0; o[b] = make_float4(0, 0, 0, 0);
+                        const uint32_t R = place(min(x0 + b * 8 * kRows, here - 1));
+                        v[b] = ld_cluster4(from + R * DP * 4 + (((c >> 2) ^ (R & 7)) << 4));
                     }
-                    float2 y[kBatch][8];
-#pragma unroll
-                    for (uint32_t s = 0; s < 8; s++)
-                        if (s < ranks)
-#pragma unroll
-                            for (uint32_t b = 0; b < kBatch; b++) y[b][s] = ld_cluster2(smem_of(ring + L::out + R[b] * 8, spread ? s : rank));
 #pragma unroll
                     for (uint32_t b = 0; b < kBatch; b++) {
-#pragma unroll
-                        for (uint32_t s = 0; s < 8; s++) if (s < ranks) M[b] = fmaxf(M[b], y[b][s].x);
-#pragma unroll
-                        for (uint32_t s = 0; s < 8; s++)
-                            if (s < ranks) { f[b][s] = y[b][s].x == -INFINITY ? (y[b][s].y == 0.0f ? 0.0f : 1.0f) : ex2(y[b][s].x - M[b]); l[b] += y[b][s].y * f[b][s]; }
-                    }
-#pragma unroll
-                    for (uint32_t s = 0; s < 8; s++)
-                        if (s < ranks) {
-                            float4 v[kBatch];
-#pragma unroll
-                            for (uint32_t b = 0; b < kBatch; b++) v[b] = ld_cluster4(smem_of(ring + R[b] * DP * 4 + (((c >> 2) ^ (R[b] & 7)) << 4), spread ? s : rank));
-#pragma unroll
-                            for (uint32_t b = 0; b < kBatch; b++)
-                                if (f[b][s] != 0.0f) { o[b].x += v[b].x * f[b][s]; o[b].y += v[b].y * f[b][s]; o[b].z += v[b].z * f[b][s]; o[b].w += v[b].w * f[b][s]; }
-                        }
-#pragma unroll
-                    for (uint32_t b = 0; b < kBatch; b++) {
-                        const uint32_t x = x0 + b * step, i = x / p.group, head = kh * p.group + x % p.group;
-                        if (x >= here || c >= D) continue;
-                        if constexpr (PREFIX) {
-                            const uint64_t at = ((uint64_t)(it.first + i) * p.heads + head) * p.splits + split;
-                            if (c == 0) p.part_ml[at] = make_float2(M[b], l[b]);
-                            *reinterpret_cast<float4 *>(p.part_o + at * D + c) = o[b];
-                        } else {
-                            const float inv = l[b] == 0.0f ? 0.0f : 1.0f / l[b];
-                            *reinterpret_cast<uint2 *>(static_cast<T *>(p.O) + (uint64_t)(it.q0 + it.first + i) * p.ldo + (uint64_t)head * D + c) =
-                                make_uint2(pack2<T>(o[b].x * inv, o[b].y * inv), pack2<T>(o[b].z * inv, o[b].w * inv));
-                        }
+                        float f;
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(weights + (min(x0 + b * 8 * kRows, x_hi - 1) - x_lo) * 32 + s * 4) : "memory");
+                        if (f != 0.0f) { o[b].x += v[b].x * f; o[b].y += v[b].y * f; o[b].z += v[b].z * f; o[b].w += v[b].w * f; }
                     }
                 }
+#pragma unroll
+                for (uint32_t b = 0; b < kBatch; b++) {
+                    const uint32_t x = x0 + b * 8 * kRows, i = x * p.group_mul >> 16, head = kh * p.group + x - i * p.group;
+                    if (x < x_hi && c < D)
+                        *reinterpret_cast<uint2 *>(static_cast<T *>(p.O) + (uint64_t)(it.q0 + it.first + i) * p.ldo + (uint64_t)head * D + c) =
+                            make_uint2(pack2<T>(o[b].x, o[b].y), pack2<T>(o[b].z, o[b].w));
+                }
+            }
+        } else if (PREFIX && ok && tile < n_tiles) {
+            // fp32 parts, through the memory of the warp's own rows of Q (their products are done), 32 channels at a
+            // time, so that stores are whole lines; a thread storing its own row touches 32 lines per instruction
+            const uint32_t buf = q_smem + tile * L::tile + (warp & 3) * 32 * 128;
+            auto at_of = [&](uint32_t R) {
+                const uint32_t q = R * p.group_mul >> 16;
+                return ((uint64_t)(it.first + tile * p.tokens + q) * p.heads + kh * p.group + R - q * p.group) * p.splits + split;
+            };
+            if (mine) p.part_ml[at_of(row)] = make_float2(m == -INFINITY ? -INFINITY : m * sc, l);
+            for (uint32_t c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                tmem_ld32(o_addr + c, o);
+                tmem_wait_ld();
+                pin32(o);
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e++)
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(buf + lane * 128 + ((e ^ (lane & 7)) << 4)), "r"(o[4 * e]), "r"(o[4 * e + 1]),
+                                 "r"(o[4 * e + 2]), "r"(o[4 * e + 3]) : "memory");
+                __syncwarp();
+#pragma unroll
+                for (uint32_t r0 = 0; r0 < 32; r0 += 4) {
+                    const uint32_t r = r0 + lane / 8, e = lane & 7, R = (warp & 3) * 32 + r;
+                    uint4 y;
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w) : "r"(buf + r * 128 + ((e ^ (r & 7)) << 4)) : "memory");
+                    if (R < p.tokens * p.group && tile * p.tokens + (R * p.group_mul >> 16) < n_here && c + e * 4 < D)
+                        *reinterpret_cast<uint4 *>(p.part_o + at_of(R) * D + c + e * 4) = y;
+                }
+                __syncwarp();
             }
         } else if (!PREFIX && ok && tile < n_tiles) {
             // The warp's rows through the memory of its own rows of Q (their products are done), so that lanes
@@ -638,7 +665,7 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
         if (__any_sync(0xffffffffu, found) && lane == 0) bad_values = 1;
     }
     __syncwarp();
-    if (warp >= 8 && spread) cluster_sync();         // the one the softmax warps pass before they join
+    if (SPLIT && warp >= 8 && spread) cluster_sync();         // the one the softmax warps pass before they join
     __syncthreads();
     if (abort_flag) {
         // a wait ran out (never in a healthy run): report, then let copies and products in flight end
@@ -655,7 +682,7 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
         }
         __syncthreads();
     }
-    if (spread) cluster_sync();              // nobody leaves while its memory is read
+    if (SPLIT && spread) cluster_sync();     // nobody leaves while its memory is read
     if (!PREFIX && bad_values && !abort_flag && rank == 0 && it.any) {
         __syncthreads();                     // over the rows just written
         for (uint32_t x = warp; x < n_here * p.group; x += kTcThreads / 32) {

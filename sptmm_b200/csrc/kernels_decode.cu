@@ -43,6 +43,9 @@ struct DecodeParams {
     const float2 *prefix_ml;
     const float *prefix_o;
     uint32_t splits;
+    // Beside the prefix's kernel only this many CTAs find an SM at once, the others when that kernel ends; `lead`:
+    // blocks that the early ones have done by then.  0: all start together.
+    uint32_t early, lead;
 };
 
 __device__ __forceinline__ uint32_t own_keys(const DecodeParams &p, uint32_t b)
@@ -149,11 +152,15 @@ k_decode(const DecodeParams p)
         if (w < warp) before += warp_sum[w];
         total += warp_sum[w];
     }
-    // no CTA between two that work may stay empty, or a unit's pieces would not be neighbours
-    const uint64_t active = min((uint64_t)gridDim.x, total);
+    // Equal runs; behind a prefix the early CTAs take `lead` blocks more than the late ones, or everything.  No CTA
+    // between two that work may stay empty, or a unit's pieces would not be neighbours.
+    const uint64_t lead = (uint64_t)p.early * p.lead;
+    const bool late = p.early && total >= lead + gridDim.x;
+    const uint64_t even = late ? total - lead : total, active = late ? gridDim.x : min((uint64_t)(p.early ? p.early : gridDim.x), total);
     if (cta >= active) { end(); return; }
+    auto start_of = [&](uint64_t c) { return even * c / active + (late ? min(c, (uint64_t)p.early) * p.lead : 0); };
     Walk walk;
-    walk.w = total * cta / active; walk.w1 = total * (cta + 1) / active;
+    walk.w = start_of(cta); walk.w1 = start_of(cta + 1);
     if (before <= walk.w && walk.w < before + mine) {
         uint64_t at = before;
         uint32_t b = b_lo;
@@ -428,10 +435,13 @@ __global__ void __launch_bounds__(128) k_decode_join(const DecodeParams p)
     *reinterpret_cast<uint2 *>(static_cast<T *>(p.O) + (uint64_t)b * p.ldo + (uint64_t)h * D + c) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
 }
 
-// How the prefix's keys are divided: one CTA per SM, a block of 128 keys at least, CTAs in clusters that join
-// their parts on chip.  `splits` clusters per item leave as many parts to k_decode_join.  A cluster of four
-// or eight needs that many free SMs of one GPC, so it is counted on 128 of the 148 SMs.
-struct PrefixPlan { uint32_t pairs, splits, cluster; };
+// How the prefix's keys are divided: over half of the SMs, while the sequences' own keys, whose number only the
+// device knows, stream on the other half (k_decode's early CTAs).  More parts shorten the prefix but every part
+// of a row is written and read once more in fp32.  Measured with 40 / 74 / 90 CTAs: 64 sequences of up to 700
+// own keys behind 8192 (20 heads over 5, 128 channels) 27.9 / 27.4 / 29.8 us (34 on all SMs, one kernel after the
+// other), 128 of up to 100 behind 16384 71.8 / 48.9 / 42.3, 16 of up to 4000 behind 2048 23.3 / 26.1 / 25.6.
+constexpr uint32_t kPrefixCtas = 74;
+struct PrefixPlan { uint32_t pairs, splits; };
 static PrefixPlan plan_prefix(uint32_t B, uint32_t kv_heads, uint32_t group, uint32_t prefix_len)
 {
     PrefixPlan pl{};
@@ -439,9 +449,8 @@ static PrefixPlan plan_prefix(uint32_t B, uint32_t kv_heads, uint32_t group, uin
     const uint32_t tokens = 128 / group, blocks = (prefix_len + kKeys - 1) / kKeys;
     pl.pairs = (B + 2 * tokens - 1) / (2 * tokens);
     const uint64_t items = (uint64_t)pl.pairs * kv_heads;
-    const uint32_t want = items >= 128 ? 1u : (uint32_t)(128 / items), parts = want < blocks ? want : blocks;
-    pl.cluster = parts >= 8 ? 8 : parts >= 4 ? 4 : parts >= 2 ? 2 : 1;
-    pl.splits = parts / pl.cluster;
+    const uint32_t want = items >= kPrefixCtas ? 1u : (uint32_t)(kPrefixCtas / items);
+    pl.splits = want < blocks ? want : blocks;
     return pl;
 }
 
@@ -469,9 +478,9 @@ static cudaError_t launch_decode(const DecodeParams &d, const TcParams &t, const
 {
     cudaError_t e;
     if (pl.splits) {
-        e = cudaFuncSetAttribute(k_attention_tc<T, DP, true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<DP>::smem);
+        e = cudaFuncSetAttribute(k_attention_tc<T, DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcLayout<DP>::smem);
         if (e != cudaSuccess) return e;
-        e = launch_clusters(pl.cluster, k_attention_tc<T, DP, true, true>, dim3(pl.pairs * t.kv_heads * pl.splits * pl.cluster), dim3(kTcThreads), TcLayout<DP>::smem, stream, pdl, t, maps[0], maps[1], maps[2]);
+        e = launch(k_attention_tc<T, DP, true>, dim3(pl.pairs * t.kv_heads * pl.splits), dim3(kTcThreads), TcLayout<DP>::smem, stream, pdl, t, maps[0], maps[1], maps[2]);
         if (e != cudaSuccess) return e;
         pdl = true;
     }
@@ -521,7 +530,7 @@ extern "C" int sptmm_attention_decode(const sptmm_decode_params *a, uint32_t fla
         return fail(SPTMM_ERR_INVALID, "%s: workspace of %llu bytes, %llu needed", who, (unsigned long long)(a->workspace ? a->workspace_bytes : 0), (unsigned long long)need);
     const uint32_t kv_heads = a->cache->kv_heads, D = a->cache->head_dim, group = a->heads / kv_heads, dtype = a->cache->dtype;
     const WorkspacePlan w = plan_workspace(a->B, a->heads, kv_heads, D, a->prefix_len);
-    if ((uint64_t)a->B * kv_heads * w.row_tiles + kMaxDecodeCtas > 0x7fffffffull || (uint64_t)w.prefix.pairs * kv_heads * w.prefix.splits > 0x7fffffffull / 8 ||
+    if ((uint64_t)a->B * kv_heads * w.row_tiles + kMaxDecodeCtas > 0x7fffffffull || (uint64_t)w.prefix.pairs * kv_heads * w.prefix.splits > 0x7fffffffull ||
         (uint64_t)a->B * a->heads > 0x7fffffffull)
         return fail(SPTMM_ERR_UNSUPPORTED, "%s: %u sequences of %u key heads in one call", who, a->B, kv_heads);
     char *ws = static_cast<char *>(a->workspace);
@@ -539,7 +548,7 @@ extern "C" int sptmm_attention_decode(const sptmm_decode_params *a, uint32_t fla
         t.Q = a->Q; t.ldq = prm.ldq; t.T = a->B; t.heads = a->heads; t.kv_heads = kv_heads; t.group = group; t.head_dim = D;
         t.tokens = 128 / group; t.group_mul = 65535 / group + 1; t.scale = prm.scale;
         t.prefix_table = a->prefix_table; t.prefix_len = a->prefix_len; t.n_pages = prm.cache.n_pages; t.page_shift = prm.cache.page_shift;
-        t.splits = w.prefix.splits; t.cluster = w.prefix.cluster;
+        t.splits = w.prefix.splits; t.cluster = 1;
         t.part_o = reinterpret_cast<float *>(ws + w.prefix_o); t.part_ml = reinterpret_cast<float2 *>(ws + w.prefix_ml);
         rc = attention_status_word(&t.status);
         if (rc != SPTMM_OK) return rc;
@@ -556,6 +565,15 @@ extern "C" int sptmm_attention_decode(const sptmm_decode_params *a, uint32_t fla
     SPTMM_CUDA_TRY(cudaGetDevice(&dev));
     SPTMM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     const uint32_t ctas = 2 * (uint32_t)sms < kMaxDecodeCtas ? 2 * (uint32_t)sms : kMaxDecodeCtas;
+    if (a->prefix_len) {
+        const uint32_t busy = w.prefix.pairs * kv_heads * w.prefix.splits, per_split = (a->prefix_len + kKeys * w.prefix.splits - 1) / (kKeys * w.prefix.splits);
+        if (busy < (uint32_t)sms) {
+            prm.early = 2 * ((uint32_t)sms - busy) < ctas ? 2 * ((uint32_t)sms - busy) : ctas;
+            // A part of the prefix takes about 5 us and 1.7 us per block of 128 keys, a late CTA another 4 us to its
+            // first keys; an early CTA gets through 64 keys of 128 channels in 1 us or less.
+            prm.lead = (8 + per_split * 12 / 5) * (D > 64 ? 1 : 2);
+        }
+    }
     const bool pdl = flags & SPTMM_LAUNCH_PDL, wide = D > 64;
     cudaError_t e;
     if (dtype == SPTMM_F16) e = wide ? launch_decode<__half, 128>(prm, t, w.prefix, maps, ctas, stream, pdl) : launch_decode<__half, 64>(prm, t, w.prefix, maps, ctas, stream, pdl);
