@@ -480,7 +480,7 @@ int sptmm_splitk_free(sptmm_splitk *s);
  *    statistics, norms and sums are fp32; a softmax weight is rounded to `dtype` before it multiplies
  *    a value, an output once at the end.
  *  - `heads` query heads share `kv_heads` key and value heads: head h reads key head
- *    h / (heads / kv_heads); heads is a multiple of kv_heads, at most 128 times it.
+ *    h / (heads / kv_heads); heads is a multiple of kv_heads, at most 128 times it, and below 65536.
  *  - head_dim is a multiple of 8 up to 128.  A row of Q holds its heads back to back (head h at
  *    h * head_dim); ld* is the number of elements between rows (0 = back to back), a multiple of 8,
  *    so that Q, K and V may be column ranges of one fused row.  Device addresses are 16-byte aligned;

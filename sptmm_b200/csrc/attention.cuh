@@ -52,7 +52,7 @@ inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 inline int check_heads(const char *who, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t dtype)
 {
     if (dtype != SPTMM_F16 && dtype != SPTMM_BF16) return fail(SPTMM_ERR_INVALID, "%s: dtype %u is neither fp16 nor bf16", who, dtype);
-    if (heads == 0 || kv_heads == 0 || heads % kv_heads || kv_heads > 65535)
+    if (heads == 0 || kv_heads == 0 || heads % kv_heads || heads > 65535)
         return fail(SPTMM_ERR_INVALID, "%s: %u query heads over %u key heads", who, heads, kv_heads);
     if (heads / kv_heads > kMaxGroup) return fail(SPTMM_ERR_UNSUPPORTED, "%s: %u query heads per key head (at most %u)", who, heads / kv_heads, kMaxGroup);
     if (head_dim == 0 || head_dim % 8) return fail(SPTMM_ERR_INVALID, "%s: head_dim %u is not a multiple of 8", who, head_dim);

@@ -6,13 +6,16 @@
 //     x *= w * rsqrt(mean(x^2) + eps)                          (query and key heads, where asked for)
 //     (a, b) -> (a cos t - b sin t, a sin t + b cos t)         t = position * inv_freq[pair]
 // and one rounding to 16 bits.  HBM bound: every input element is read once and every output element
-// written once.  A CTA takes one token, because its heads share the cosines; a group of LPH lanes
-// takes a head, each lane four neighbouring channels (16-byte loads of fp32, 8-byte of 16-bit rows),
-// so the mean is a butterfly over the group and a pair's partner lies in the same lane (interleaved
-// pairs) or one shuffle away (pairs half the rotated range apart).  The loads of four heads per group
-// are in flight while the angles are formed: position * inv_freq / 2 pi in 64 bits, reduced to a
-// fraction of a turn, then sincospif in 32 -- at position 131071 a product in 32 bits would already be
-// off by 2^-8 radians.
+// written once.  A CTA takes one token, because its heads share the cosines.  A group of 16 lanes (8 up to
+// 64 channels) takes a head, eight channels to a lane and chosen so that a channel and its partner meet in
+// one lane whichever way pairs are formed: only the mean needs shuffles, and a lane's four cosines serve
+// all of its heads.  All loads of a token are in flight while the angles are formed:
+// position * inv_freq / 2 pi in 64 bits, reduced to a fraction of a turn, then sincospif in 32 -- at
+// position 131071 a product in 32 bits would already be off by 2^-8 radians.
+// Measured on 8192 tokens of 20 + 5 + 5 heads of 128 channels, fp32 -> bf16 (210 MB): 36 us, 5.8 TB/s, 0.89
+// of the copy rate, with five CTAs per SM (48 registers); four or six: 38.6, 36.6; eight (32 registers):
+// 47.9.  Four channels per lane with partners shuffled: 57.  CTAs that walk over tokens and fetch the next
+// one's heads ahead: 64, for the registers that takes.  One to sixteen tokens: 2.9 us, a launch.
 #include "attention.cuh"
 
 namespace sptmm {
@@ -25,7 +28,6 @@ struct RotateParams {
     CacheView cache;
     uint64_t ldx, ldq, ldk, ldv;
     uint32_t heads, kv_heads, head_dim, rot_dim, interleaved, has_cache;
-    uint32_t heads_per_cta;                  // heads (q, k and v counted alike) along grid.y
     float eps;
     double inv_freq[kMaxHeadDim / 2];
 };
@@ -45,113 +47,125 @@ template <> __device__ __forceinline__ void to_float<float>(const uint4 &r, floa
     x[0] = __uint_as_float(r.x); x[1] = __uint_as_float(r.y); x[2] = __uint_as_float(r.z); x[3] = __uint_as_float(r.w);
 }
 
-constexpr int kRotateThreads = 256, kRotateBatch = 4;
+constexpr int kRotateThreads = 256, kRotateBatch = 2;
 
-// LPH lanes of four channels each hold a head: 16 up to 64 channels, 32 beyond.
+// LPH lanes of eight channels each hold a head: 8 up to 64 channels, 16 beyond.  grid.x: tokens, grid.y: batches
+// of GROUPS * 2 of a token's heads.
 template <typename TI, typename TO, int LPH>
-__global__ void __launch_bounds__(kRotateThreads) k_rotate(const __grid_constant__ RotateParams p)
+__global__ void __launch_bounds__(kRotateThreads, 5) k_rotate(const __grid_constant__ RotateParams p)
 {
+    using Raw = typename In4<TI>::raw;
     __shared__ float2 turn[kMaxHeadDim / 2];                 // (cos, sin) of the token's angles
-    constexpr int GROUPS = kRotateThreads / LPH;
-    const uint32_t t = blockIdx.x, tid = threadIdx.x, c = tid % LPH, group = tid / LPH;
-    const uint32_t D = p.head_dim, rot = p.rot_dim, n_heads = p.heads + 2 * p.kv_heads;
-    const uint32_t first = blockIdx.y * p.heads_per_cta, last = min(n_heads, first + p.heads_per_cta);
-    const bool active = c * 4 < D;
+    constexpr uint32_t GROUPS = kRotateThreads / LPH;
+    const uint32_t tid = threadIdx.x, lane = tid % LPH, group = tid / LPH, mask = ((1u << LPH) - 1) << (tid & 31 & ~(LPH - 1));
+    const uint32_t D = p.head_dim, rot = p.rot_dim, qk_heads = p.heads + p.kv_heads, n_heads = qk_heads + p.kv_heads;
+    const uint32_t t = blockIdx.x, first = blockIdx.y * GROUPS * kRotateBatch;
+    // This lane's channels: a .. a + 4 and b .. b + 4, the partners of one another where pairs lie rot / 2 apart
+    const bool active = lane * 8 < D, apart = !p.interleaved && lane * 8 < rot;
+    const uint32_t a = apart ? lane * 4 : lane * 8, b = apart ? rot / 2 + lane * 4 : lane * 8 + 4;
     pdl_launch_dependents();
     pdl_wait_prior_grid();
+    const int32_t pos = tid < rot / 2 ? p.positions[t] : 0;
+    const int32_t slot = p.has_cache ? p.slots[t] : -1;
+    const bool cached = slot >= 0 && ((uint32_t)slot >> p.cache.page_shift) < p.cache.n_pages;
     const TI *row = static_cast<const TI *>(p.X) + (uint64_t)t * p.ldx;
-    for (uint32_t h0 = first; h0 < last; h0 += GROUPS * kRotateBatch) {
-        typename In4<TI>::raw raw[kRotateBatch];
+    Raw raw[kRotateBatch][2];
 #pragma unroll
-        for (int u = 0; u < kRotateBatch; u++) {
-            const uint32_t h = h0 + u * GROUPS + group;
-            raw[u] = typename In4<TI>::raw{};
-            if (h < last && active) raw[u] = __ldcs(reinterpret_cast<const typename In4<TI>::raw *>(row + (uint64_t)h * D + c * 4));
+    for (uint32_t u = 0; u < kRotateBatch; u++) {
+        const uint32_t h = first + u * GROUPS + group;
+        raw[u][0] = raw[u][1] = Raw{};
+        if (h < n_heads && active) {
+            raw[u][0] = __ldcs(reinterpret_cast<const Raw *>(row + (uint64_t)h * D + a));
+            raw[u][1] = __ldcs(reinterpret_cast<const Raw *>(row + (uint64_t)h * D + b));
         }
-        if (h0 == first) {
-            if (tid < rot / 2) {
-                double turns = (double)p.positions[t] * p.inv_freq[tid] * 0.15915494309189533577;      // 1 / (2 pi)
-                turns -= rint(turns);
-                float s, co;
-                sincospif(2.0f * (float)turns, &s, &co);
-                turn[tid] = make_float2(co, s);
-            }
-            __syncthreads();
-        }
-        const int32_t slot = p.has_cache ? p.slots[t] : -1;
-        const bool cached = slot >= 0 && ((uint32_t)slot >> p.cache.page_shift) < p.cache.n_pages;
+    }
+    if (tid < rot / 2) {
+        double turns = (double)pos * p.inv_freq[tid] * 0.15915494309189533577;                 // 1 / (2 pi)
+        turns -= rint(turns);
+        float s, co;
+        sincospif(2.0f * (float)turns, &s, &co);
+        turn[tid] = make_float2(co, s);
+    }
+    __syncthreads();
+    // the four pairs of this lane, the same for every head
+    float4 cs[2] = {};
+    if (lane * 8 < rot) {
+        cs[0] = *reinterpret_cast<const float4 *>(&turn[lane * 4]);
+        cs[1] = *reinterpret_cast<const float4 *>(&turn[lane * 4 + 2]);
+    }
 #pragma unroll
-        for (int u = 0; u < kRotateBatch; u++) {
-            const uint32_t h = h0 + u * GROUPS + group;
-            float x[4];
-            to_float<TI>(raw[u], x);
-            if (h < p.heads + p.kv_heads) {                  // a query or key head; the same for all lanes of the group
+    for (uint32_t u = 0; u < kRotateBatch; u++) {
+        const uint32_t h = first + u * GROUPS + group;
+        float x[4], y[4];
+        to_float<TI>(raw[u][0], x);
+        to_float<TI>(raw[u][1], y);
+        if (h < qk_heads) {                              // a query or key head; the same for all lanes of the group
+            if (h < p.heads ? p.q_norm != nullptr : p.k_norm != nullptr) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) ss += x[i] * x[i] + y[i] * y[i];
+#pragma unroll
+                for (int o = LPH / 2; o; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+                const float r = rsqrtf(ss / (float)D + p.eps);
                 const float *w = h < p.heads ? p.q_norm : p.k_norm;
-                if (w) {
-                    float ss = x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3];
-#pragma unroll
-                    for (int o = LPH / 2; o; o >>= 1) ss += __shfl_xor_sync(LPH == 32 ? 0xffffffffu : 0xffffu << (tid & 16), ss, o);
-                    const float r = rsqrtf(ss / (float)D + p.eps);
-                    const float4 g = active ? *reinterpret_cast<const float4 *>(w + c * 4) : make_float4(0, 0, 0, 0);
+                if (active) {
+                    const float4 g = *reinterpret_cast<const float4 *>(w + a), k = *reinterpret_cast<const float4 *>(w + b);
                     x[0] *= r * g.x; x[1] *= r * g.y; x[2] *= r * g.z; x[3] *= r * g.w;
-                }
-                if (rot) {
-                    if (p.interleaved) {
-                        if (c * 4 < rot) {
-                            const float2 a = turn[c * 2], b = turn[c * 2 + 1];
-                            const float x0 = x[0], x2 = x[2];
-                            x[0] = x0 * a.x - x[1] * a.y; x[1] = x0 * a.y + x[1] * a.x;
-                            x[2] = x2 * b.x - x[3] * b.y; x[3] = x2 * b.y + x[3] * b.x;
-                        }
-                    } else {
-                        const uint32_t half = rot / 8;       // lanes per half of the rotated range
-                        const uint32_t other = c < half ? c + half : c < 2 * half ? c - half : c;
-                        float y[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) y[i] = __shfl_sync(LPH == 32 ? 0xffffffffu : 0xffffu << (tid & 16), x[i], other, LPH);
-                        if (c < 2 * half) {
-                            const uint32_t pair = (c < half ? c : c - half) * 4;
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                const float2 a = turn[pair + i];
-                                x[i] = c < half ? x[i] * a.x - y[i] * a.y : y[i] * a.y + x[i] * a.x;
-                            }
-                        }
-                    }
+                    y[0] *= r * k.x; y[1] *= r * k.y; y[2] *= r * k.z; y[3] *= r * k.w;
                 }
             }
-            if (h >= last || !active) continue;
-            const uint2 w = make_uint2(pack2<TO>(x[0], x[1]), pack2<TO>(x[2], x[3]));
-            if (h < p.heads) {
-                *reinterpret_cast<uint2 *>(static_cast<TO *>(p.Q) + (uint64_t)t * p.ldq + (uint64_t)h * D + c * 4) = w;
+            const float co[4] = {cs[0].x, cs[0].z, cs[1].x, cs[1].z}, si[4] = {cs[0].y, cs[0].w, cs[1].y, cs[1].w};
+            if (lane * 8 >= rot) {
+                // not rotated
+            } else if (p.interleaved) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const float x0 = x[2 * i], y0 = y[2 * i];
+                    x[2 * i] = x0 * co[i] - x[2 * i + 1] * si[i]; x[2 * i + 1] = x0 * si[i] + x[2 * i + 1] * co[i];
+                    y[2 * i] = y0 * co[2 + i] - y[2 * i + 1] * si[2 + i]; y[2 * i + 1] = y0 * si[2 + i] + y[2 * i + 1] * co[2 + i];
+                }
             } else {
-                const bool is_v = h >= p.heads + p.kv_heads;
-                const uint32_t kh = h - p.heads - (is_v ? p.kv_heads : 0);
-                if (p.K) {
-                    TO *o = static_cast<TO *>(is_v ? p.V : p.K) + (uint64_t)t * (is_v ? p.ldv : p.ldk);
-                    *reinterpret_cast<uint2 *>(o + (uint64_t)kh * D + c * 4) = w;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float x0 = x[i];
+                    x[i] = x0 * co[i] - y[i] * si[i]; y[i] = x0 * si[i] + y[i] * co[i];
                 }
-                if (cached) {
-                    TO *o = static_cast<TO *>(is_v ? p.cache.v : p.cache.k);
-                    o += p.cache.at((uint32_t)slot >> p.cache.page_shift, kh, (uint32_t)slot & (p.cache.page_size() - 1));
-                    *reinterpret_cast<uint2 *>(o + c * 4) = w;
-                }
+            }
+        }
+        if (h < n_heads && active) {
+            const uint2 w0 = make_uint2(pack2<TO>(x[0], x[1]), pack2<TO>(x[2], x[3])), w1 = make_uint2(pack2<TO>(y[0], y[1]), pack2<TO>(y[2], y[3]));
+            auto store = [&](TO *o) { *reinterpret_cast<uint2 *>(o + a) = w0; *reinterpret_cast<uint2 *>(o + b) = w1; };
+            if (h < p.heads) {
+                store(static_cast<TO *>(p.Q) + (uint64_t)t * p.ldq + (uint64_t)h * D);
+            } else {
+                const bool is_v = h >= qk_heads;
+                const uint32_t kh = h - (is_v ? qk_heads : p.heads);
+                if (p.K) store(static_cast<TO *>(is_v ? p.V : p.K) + (uint64_t)t * (is_v ? p.ldv : p.ldk) + (uint64_t)kh * D);
+                if (cached)
+                    store(static_cast<TO *>(is_v ? p.cache.v : p.cache.k) +
+                          p.cache.at((uint32_t)slot >> p.cache.page_shift, kh, (uint32_t)slot & (p.cache.page_size() - 1)));
             }
         }
     }
 }
 
-template <typename TI, typename TO>
-static cudaError_t launch_rotate(const RotateParams &prm, dim3 grid, void *stream, bool pdl)
+template <typename TI, typename TO, int LPH>
+static cudaError_t launch_rotate(const RotateParams &prm, uint32_t T, void *stream, bool pdl)
 {
-    if (prm.head_dim <= 64) return launch(k_rotate<TI, TO, 16>, grid, dim3(kRotateThreads), 0, stream, pdl, prm);
-    return launch(k_rotate<TI, TO, 32>, grid, dim3(kRotateThreads), 0, stream, pdl, prm);
+    constexpr uint32_t heads = kRotateThreads / LPH * kRotateBatch;
+    return launch(k_rotate<TI, TO, LPH>, dim3(T, (prm.heads + 2 * prm.kv_heads + heads - 1) / heads), dim3(kRotateThreads), 0, stream, pdl, prm);
+}
+
+template <typename TI, typename TO>
+static cudaError_t launch_rotate(const RotateParams &prm, uint32_t T, void *stream, bool pdl)
+{
+    return prm.head_dim <= 64 ? launch_rotate<TI, TO, 8>(prm, T, stream, pdl) : launch_rotate<TI, TO, 16>(prm, T, stream, pdl);
 }
 
 template <typename TI>
-static cudaError_t launch_rotate_to(const RotateParams &prm, uint32_t dtype, dim3 grid, void *stream, bool pdl)
+static cudaError_t launch_rotate_to(const RotateParams &prm, uint32_t dtype, uint32_t T, void *stream, bool pdl)
 {
-    return dtype == SPTMM_F16 ? launch_rotate<TI, __half>(prm, grid, stream, pdl) : launch_rotate<TI, __nv_bfloat16>(prm, grid, stream, pdl);
+    return dtype == SPTMM_F16 ? launch_rotate<TI, __half>(prm, T, stream, pdl) : launch_rotate<TI, __nv_bfloat16>(prm, T, stream, pdl);
 }
 
 }  // namespace sptmm
@@ -197,13 +211,11 @@ extern "C" int sptmm_rotate_heads(const sptmm_rotate_params *a, uint32_t flags, 
     prm.heads = a->heads; prm.kv_heads = a->kv_heads; prm.head_dim = a->head_dim; prm.rot_dim = a->rot_dim;
     prm.interleaved = a->interleaved ? 1 : 0; prm.has_cache = a->cache ? 1 : 0; prm.eps = a->eps;
     for (uint32_t i = 0; i < a->rot_dim / 2; i++) prm.inv_freq[i] = a->inv_freq[i];
-    prm.heads_per_cta = a->heads + 2 * a->kv_heads;
-    const dim3 grid(a->T);
     const bool pdl = flags & SPTMM_LAUNCH_PDL;
     cudaError_t e;
-    if (a->in_dtype == SPTMM_F32) e = launch_rotate_to<float>(prm, a->dtype, grid, stream, pdl);
-    else if (a->in_dtype == SPTMM_F16) e = launch_rotate_to<__half>(prm, a->dtype, grid, stream, pdl);
-    else e = launch_rotate_to<__nv_bfloat16>(prm, a->dtype, grid, stream, pdl);
+    if (a->in_dtype == SPTMM_F32) e = launch_rotate_to<float>(prm, a->dtype, a->T, stream, pdl);
+    else if (a->in_dtype == SPTMM_F16) e = launch_rotate_to<__half>(prm, a->dtype, a->T, stream, pdl);
+    else e = launch_rotate_to<__nv_bfloat16>(prm, a->dtype, a->T, stream, pdl);
     if (e != cudaSuccess) return fail(SPTMM_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     return SPTMM_OK;
 }

@@ -50,6 +50,7 @@ INVALID, UNSUPPORTED = -1, -3
     (INVALID, "query heads", dict(heads=0)),
     (INVALID, "query heads", dict(kv_heads=0)),
     (INVALID, "query heads", dict(heads=5)),
+    (INVALID, "query heads", dict(heads=65536, kv_heads=1024)),
     (UNSUPPORTED, "per key head", dict(heads=258)),
     (INVALID, "multiple of 8", dict(head_dim=12)),
     (INVALID, "multiple of 8", dict(head_dim=0)),
