@@ -521,7 +521,9 @@ def rotate_heads(QKV, T: int, heads: int, kv_heads: int, head_dim: int, position
     if inv_freq is not None:
         f = np.ascontiguousarray(inv_freq, dtype=np.float64)
         pairs = f.size
-    p = _pack_rotate(_addr(QKV), _addr(q_norm), _addr(k_norm), f.__array_interface__["data"][0] if pairs else 0, _addr(positions),
+        if not f.flags.writeable:
+            f = f.copy()                     # from_buffer below wants a writeable array; a third of the time of f.ctypes
+    p = _pack_rotate(_addr(QKV), _addr(q_norm), _addr(k_norm), C.addressof(C.c_char.from_buffer(f)) if pairs else 0, _addr(positions),
                      _addr(slots), _addr(Q), _addr(K), _addr(V), cache.address if cache is not None else 0, ldqkv, ldq, ldk, ldv,
                      T, heads, kv_heads, head_dim, in_dtype, dtype, 2 * pairs, 1 if interleaved else 0, eps)
     check(lib.sptmm_rotate_heads(p, flags, stream))

@@ -409,9 +409,9 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                 }
             }
             // the CTAs of the cluster share the rows: first every row's weights, a thread per row, then the rows,
-            // eight of a warp at a time (half a warp to a row up to 64 channels)
+            // four of a warp at a time from four CTAs at a time (half a warp to a row up to 64 channels)
             cluster_sync();
-            constexpr uint32_t kLanes = DP / 4, kRows = 32 / kLanes, kBatch = 8;
+            constexpr uint32_t kLanes = DP / 4, kRows = 32 / kLanes, kBatch = 4, kFrom = 4;
             const uint32_t ranks = p.cluster, used = p.tokens * p.group, here = n_here * p.group, weights = q_smem;      // weights: Q is done with; 8 factors and 1 / l per row
             auto place = [&](uint32_t x) { return x + (x >= used ? 128 - used : 0); };       // row x of those in use, counted over both tiles
             const uint32_t share = (here + ranks - 1) / ranks, x_lo = rank * share, x_hi = min(here, x_lo + share);
@@ -441,20 +441,26 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                 float4 o[kBatch];
 #pragma unroll
                 for (uint32_t b = 0; b < kBatch; b++) o[b] = make_float4(0, 0, 0, 0);
-                for (uint32_t s = 0; s < ranks; s++) {
-                    const uint32_t from = smem_of(ring, s);
-                    float4 v[kBatch];
+                for (uint32_t s0 = 0; s0 < ranks; s0 += kFrom) {
+                    float4 v[kFrom][kBatch];
 #pragma unroll
-                    for (uint32_t b = 0; b < kBatch; b++) {
-                        const uint32_t R = place(min(x0 + b * 8 * kRows, here - 1));
-                        v[b] = ld_cluster4(from + R * DP * 4 + (((c >> 2) ^ (R & 7)) << 4));
+                    for (uint32_t k = 0; k < kFrom; k++) {
+                        const uint32_t from = smem_of(ring, min(s0 + k, ranks - 1));
+#pragma unroll
+                        for (uint32_t b = 0; b < kBatch; b++) {
+                            const uint32_t R = place(min(x0 + b * 8 * kRows, here - 1));
+                            if (s0 + k < ranks) v[k][b] = ld_cluster4(from + R * DP * 4 + (((c >> 2) ^ (R & 7)) << 4));
+                        }
                     }
 #pragma unroll
-                    for (uint32_t b = 0; b < kBatch; b++) {
-                        float f;
-                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(weights + (min(x0 + b * 8 * kRows, x_hi - 1) - x_lo) * 32 + s * 4) : "memory");
-                        if (f != 0.0f) { o[b].x += v[b].x * f; o[b].y += v[b].y * f; o[b].z += v[b].z * f; o[b].w += v[b].w * f; }
-                    }
+                    for (uint32_t k = 0; k < kFrom; k++)
+                        if (s0 + k < ranks)
+#pragma unroll
+                            for (uint32_t b = 0; b < kBatch; b++) {
+                                float f;
+                                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(weights + (min(x0 + b * 8 * kRows, x_hi - 1) - x_lo) * 32 + (s0 + k) * 4) : "memory");
+                                if (f != 0.0f) { o[b].x += v[k][b].x * f; o[b].y += v[k][b].y * f; o[b].z += v[k][b].z * f; o[b].w += v[k][b].w * f; }
+                            }
                 }
 #pragma unroll
                 for (uint32_t b = 0; b < kBatch; b++) {
