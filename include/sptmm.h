@@ -490,7 +490,9 @@ int sptmm_splitk_free(sptmm_splitk *s);
  *    What they name beyond a buffer's end (a slot or page outside the cache, an offset outside its
  *    rows) is left out, not followed.
  *  - A query without any visible key gives a row of zeros.
- *  - No call allocates or synchronises.  SPTMM_LAUNCH_PDL in `flags` as for the matmuls. */
+ *  - No call allocates or synchronises; all may be captured into a graph (like every kernel of a library,
+ *    theirs are loaded by the first call on a device, which is best made before a capture).
+ *    SPTMM_LAUNCH_PDL in `flags` as for the matmuls. */
 
 /* A paged cache.  Element (page p, key head h, slot s, channel d) of k or v lies at
  *     p * page_stride + (h * page_size + s) * head_dim + d.

@@ -48,6 +48,7 @@ struct CacheView {
 };
 
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+inline bool aligned4(const void *p) { return ((uintptr_t)p & 3) == 0; }       // index arrays
 
 inline int check_heads(const char *who, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t dtype)
 {

@@ -525,6 +525,7 @@ extern "C" int sptmm_attention_decode(const sptmm_decode_params *a, uint32_t fla
     if (!a->Q || !a->O || !a->lengths || (a->max_pages && !a->table) || (a->prefix_len && !a->prefix_table))
         return fail(SPTMM_ERR_INVALID, "%s: null pointer", who);
     if (!aligned16(a->Q) || !aligned16(a->O) || !aligned16(a->workspace)) return fail(SPTMM_ERR_INVALID, "%s: an address is not 16-byte aligned", who);
+    if (!aligned4(a->lengths) || !aligned4(a->table) || !aligned4(a->prefix_table)) return fail(SPTMM_ERR_INVALID, "%s: an index array is not 4-byte aligned", who);
     const uint64_t need = sptmm_attention_decode_workspace(a->B, a->heads, a->cache->kv_heads, a->cache->head_dim, a->prefix_len);
     if (!a->workspace || a->workspace_bytes < need)
         return fail(SPTMM_ERR_INVALID, "%s: workspace of %llu bytes, %llu needed", who, (unsigned long long)(a->workspace ? a->workspace_bytes : 0), (unsigned long long)need);

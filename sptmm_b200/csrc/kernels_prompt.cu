@@ -82,6 +82,7 @@ extern "C" int sptmm_attention_prompt(const sptmm_prompt_params *a, uint32_t fla
     if (!a->Q || !a->O || !a->q_offsets || !a->k_offsets || (a->Tk && (!a->K || !a->V))) return fail(SPTMM_ERR_INVALID, "%s: null pointer", who);
     for (const void *x : {a->Q, a->K, a->V, (const void *)a->O})
         if (!aligned16(x)) return fail(SPTMM_ERR_INVALID, "%s: an address is not 16-byte aligned", who);
+    if (!aligned4(a->q_offsets) || !aligned4(a->k_offsets)) return fail(SPTMM_ERR_INVALID, "%s: an index array is not 4-byte aligned", who);
     prm.Q = a->Q; prm.K = a->K; prm.V = a->V; prm.O = a->O; prm.q_off = a->q_offsets; prm.k_off = a->k_offsets;
     prm.n_seqs = a->n_seqs; prm.T = a->T; prm.Tk = a->Tk; prm.heads = a->heads; prm.kv_heads = a->kv_heads; prm.group = a->heads / a->kv_heads;
     prm.head_dim = a->head_dim; prm.causal = a->causal ? 1 : 0;

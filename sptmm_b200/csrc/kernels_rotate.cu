@@ -206,6 +206,7 @@ extern "C" int sptmm_rotate_heads(const sptmm_rotate_params *a, uint32_t flags, 
     if (!a->QKV || !a->Q || (a->rot_dim && !a->positions)) return fail(SPTMM_ERR_INVALID, "%s: null pointer", who);
     for (const void *x : {a->QKV, (const void *)a->Q, (const void *)a->K, (const void *)a->V, (const void *)a->q_norm, (const void *)a->k_norm})
         if (!aligned16(x)) return fail(SPTMM_ERR_INVALID, "%s: an address is not 16-byte aligned", who);
+    if (!aligned4(a->positions) || !aligned4(a->slots)) return fail(SPTMM_ERR_INVALID, "%s: an index array is not 4-byte aligned", who);
     prm.X = a->QKV; prm.q_norm = a->q_norm; prm.k_norm = a->k_norm; prm.positions = a->positions; prm.slots = a->slots;
     prm.Q = a->Q; prm.K = a->K; prm.V = a->V;
     prm.heads = a->heads; prm.kv_heads = a->kv_heads; prm.head_dim = a->head_dim; prm.rot_dim = a->rot_dim;

@@ -85,6 +85,8 @@ def test_shapes_types_strides(call, code, text, kw):
     (INVALID, "ldqkv", dict(ldqkv=1026, in_dtype=sp.F16)),
     (INVALID, "null pointer", dict(positions=None)),
     (INVALID, "null pointer", dict(QKV=0)),
+    (INVALID, "4-byte aligned", dict(positions=A + 2)),
+    (INVALID, "4-byte aligned", dict(slots=A + 1, cache=cache())),
     (INVALID, "16-byte aligned", dict(q_norm=A + 4)),
 ])
 def test_rotate_refusals(code, text, kw):
@@ -95,6 +97,7 @@ def test_rotate_refusals(code, text, kw):
     (INVALID, "null pointer", dict(q_offsets=0)),
     (INVALID, "null pointer", dict(k_offsets=0)),
     (INVALID, "null pointer", dict(V=None)),
+    (INVALID, "4-byte aligned", dict(k_offsets=A + 2)),
     (INVALID, "T=", dict(T=1 << 30)),
     (INVALID, "Tk=", dict(Tk=1 << 30)),
     (UNSUPPORTED, "sequences", dict(n_seqs=65537)),
@@ -129,6 +132,8 @@ def test_prompt_refusals(code, text, kw):
     (INVALID, "16-byte aligned", dict(workspace=A + 8)),
     (INVALID, "workspace", dict(workspace=None)),
     (INVALID, "workspace", dict(workspace_bytes=15)),
+    (INVALID, "4-byte aligned", dict(table=A + 2)),
+    (INVALID, "4-byte aligned", dict(lengths=A + 3)),
     (INVALID, "ldq", dict(ldq=100)),
     (INVALID, "ldo", dict(ldo=514)),
     (INVALID, "flags", dict(flags=64)),

@@ -671,3 +671,120 @@ def test_attention_between_the_ternary_products_of_a_layer():
             want, tol = attend(q[last[s]].view(1, H, D), k[a:a + lens[s]].view(-1, Hk, D), v[a:a + lens[s]].view(-1, Hk, D), sp.F16, D ** -0.5, False)
             check(got[4][s].view(1, H, D), want, tol)
             check(whole[4][last[s]].view(1, H, D), want, tol)
+
+
+def test_programmatic_launches_in_a_row():
+    """rotate -> decode behind a prefix, and rotate -> prompt, with SPTMM_LAUNCH_PDL on one stream: every call
+    reads what the one before it wrote, over and over into the same buffers."""
+    H, Hk, D, page, B, dtype = 8, 2, 128, 16, 6, sp.F16
+    lengths, prefix = [5, 40, 1, 300, 17, 64], 270
+    side = torch.cuda.Stream()
+
+    def program(flags, rounds):
+        b = Batch(lengths, prefix, H, Hk, D, dtype, page, seed=5)
+        new = [b.rows[i][(n - 1) // page] * page + (n - 1) % page for i, n in enumerate(lengths)]       # the slot of every sequence's last key
+        slots, pos = i32(new), i32([n + prefix - 1 for n in lengths])
+        inv = np.array([10000.0 ** (-i / 64) for i in range(64)])
+        off, pq = i32([0, 2, 6]), torch.zeros((B, H * D), dtype=torch.float16, device="cuda")
+        pk, pv, po = (torch.zeros((B, n * D), dtype=torch.float16, device="cuda") for n in (Hk, Hk, H))
+        outs = []
+        xs = [randn(50 + r, B, (H + 2 * Hk) * D, dtype=sp.F32) for r in range(rounds)]
+        keep = [(torch.zeros_like(b.out), torch.zeros_like(po)) for _ in range(rounds)]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for r in range(rounds):
+                s = side.cuda_stream
+                sp.rotate_heads(xs[r], B, H, Hk, D, pos, inv, b.q, dtype=dtype, K=pk, V=pv, cache=b.cache, slots=slots, flags=flags, stream=s)
+                b.call(s, flags)
+                keep[r][0].copy_(b.out)
+                sp.rotate_heads(xs[r], B, H, Hk, D, pos, inv, pq, dtype=dtype, K=pk, V=pv, flags=flags, stream=s)
+                sp.attention_prompt(pq, pk, pv, po, off, off, 2, B, B, H, Hk, D, dtype=dtype, flags=flags, stream=s)
+                keep[r][1].copy_(po)
+        torch.cuda.synchronize()
+        return keep
+
+    plain, pdl = program(0, 12), program(sp.LAUNCH_PDL, 12)
+    for a, b in zip(plain, pdl):
+        assert torch.isfinite(a[0]).all() and torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert not torch.equal(plain[0][0], plain[1][0])
+
+
+def test_two_streams_at_once():
+    """Calls on two streams, each with a workspace of its own, do not disturb one another."""
+    jobs = [Batch([900, 3, 50], 500, 8, 2, 128, sp.F16, 16, seed=1), Batch([20, 1200, 7, 64], 0, 8, 2, 128, sp.F16, 32, seed=2)]
+    want = []
+    for j in jobs:
+        j.call()
+        torch.cuda.synchronize()
+        want.append(j.out.clone())
+        j.verify()
+    T = 700
+    q, k, v = randn(1, T, 8, 128), randn(2, T, 2, 128), randn(3, T, 2, 128)
+    o, off = torch.zeros_like(q), i32([0, 300, 700])
+    prompt = lambda stream: sp.attention_prompt(q, k, v, o, off, off, 2, T, T, 8, 2, 128, stream=stream)
+    prompt(0)
+    torch.cuda.synchronize()
+    first = o.clone()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(20):
+        for s, j in zip(streams, jobs):
+            j.call(s.cuda_stream)
+        prompt(streams[2].cuda_stream)
+    torch.cuda.synchronize()
+    for j, w in zip(jobs, want):
+        assert torch.equal(j.out, w)
+    assert torch.equal(o, first)
+
+
+def test_decode_many_sequences():
+    rng = np.random.default_rng(1)
+    lengths = rng.integers(0, 40, size=1500).tolist()
+    for prefix in (0, 64):
+        b = Batch(lengths, prefix, 2, 1, 64, sp.F16, 16)
+        b.call()
+        torch.cuda.synchronize()
+        for i in list(range(0, 1500, 97)) + [1499]:
+            check(b.out[i:i + 1], *b.want(i))
+
+
+@TYPES
+def test_decode_a_row_that_is_not_finite_stays_alone(dtype):
+    for prefix in (0, 200):
+        b = Batch([100, 33, 70], prefix, 4, 1, 128, dtype, 16)
+        b.call()
+        torch.cuda.synchronize()
+        clean = b.out.clone()
+        b.q[1, 128:256] = NAN                                    # head 1 of sequence 1
+        b.call()
+        torch.cuda.synchronize()
+        assert torch.isnan(b.out[1, 1]).all()
+        b.out[1, 1] = clean[1, 1]
+        want = [b.want(i) for i in (0, 2)]
+        check(b.out[0:1], *want[0])
+        check(b.out[2:3], *want[1])
+        assert torch.isfinite(b.out).all()
+
+
+def test_prompt_clusters_and_long_keys():
+    """Few queries over many keys, so that CTAs of a cluster share them: the same rows as query by query."""
+    for H, Hk, D, n, m in ((4, 1, 128, 70, 3000), (20, 5, 128, 33, 2100), (2, 2, 64, 300, 1500), (7, 1, 80, 40, 2500)):
+        q, k, v = randn(1, n, H, D, scale=1.5), randn(2, m, Hk, D), randn(3, m, Hk, D)
+        out = torch.zeros_like(q)
+        sp.attention_prompt(q, k, v, out, i32([0, n]), i32([0, m]), 1, n, m, H, Hk, D)
+        torch.cuda.synchronize()
+        for i in (0, 1, n // 2, n - 1):
+            top = i + m - n + 1
+            want, tol = attend(q[i:i + 1], k[:top], v[:top], sp.F16, D ** -0.5, False)
+            check(out[i:i + 1], want, tol)
+        v[m - n + 20, 0, 3] = NAN                                # a key that the queries from 20 on see
+        sp.attention_prompt(q, k, v, out, i32([0, n]), i32([0, m]), 1, n, m, H, Hk, D)
+        torch.cuda.synchronize()
+        g = H // Hk
+        assert torch.isfinite(out[:20]).all() and torch.isnan(out[20:, :g, 3]).all() and torch.isfinite(out[20:, :, 4:]).all()
+        for i in (0, 19):
+            top = i + m - n + 1
+            check(out[i:i + 1], *attend(q[i:i + 1], k[:top], v[:top], sp.F16, D ** -0.5, False))
+
+
+def test_no_wait_ran_out():
+    assert sp.attention_status() == 0
