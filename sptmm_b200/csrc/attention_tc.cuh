@@ -615,20 +615,23 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                 __syncwarp();
             };
             auto full = [&](uint32_t x) { return mbar_wait_warp(b_full + 8 * (x % L::stages), x / L::stages & 1, abort_word); };
-            // A wait costs a hundred cycles even when there is nothing to wait for: those for loads come
-            // right behind an issued product, while it runs.
+            // A wait costs one or two hundred cycles even when there is nothing to wait for, a commit as much: those for
+            // loads stand behind products just issued, and nothing stands between the last product of a step and
+            // the wait for the first weights of the next.
+            auto values_in = [&](uint32_t i) { return full(2 * i + 1) && (i + 1 < n || !cut || mbar_wait_warp(b_fix, 0, abort_word)); };
             ok = full(0);
             for (uint32_t t = 0; t < n_tiles && ok; t++) {
                 ok = mbar_wait_warp(b_q + 8 * t, 0, abort_word);
                 if (ok) { tc_fence_after(); scores(t, 0); }
             }
             if (ok && leader) tc_commit(b_empty);
-            ok = ok && full(1);
+            ok = ok && values_in(0) && (n == 1 || full(2));
             for (uint32_t i = 0; i < n && ok; i++) {
                 const bool last = i + 1 == n;
-                if (last && cut) ok = mbar_wait_warp(b_fix, 0, abort_word);
                 const uint32_t vb = slot_lo(ring + (2 * i + 1) % L::stages * L::tile, 16384);
-                for (uint32_t t = 0; t < n_tiles && ok; t++) {
+#pragma unroll
+                for (uint32_t t = 0; t < 2; t++) {
+                    if (t >= n_tiles || !ok) break;
 #pragma unroll
                     for (uint32_t half = 0; half < 2; half++) {                      // O_t += P_t V, sixteen keys at a time
                         ok = ok && mbar_wait_warp(b_p + 16 * t + 8 * half, i & 1, abort_word);
@@ -638,20 +641,19 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
 #pragma unroll
                             for (uint32_t k = 0; k < 4; k++)
                                 mma_ts(tm + 256 + t * DP, tm + t * 128 + (4 * half + k) * 8, vb + (4 * half + k) * 128, v_hi, desc_o, i > 0 || half > 0 || k > 0);
+                            if (t == 0 && half == 0 && i > 0) {                         // what the step before read
+                                tc_commit(b_empty + 8 * ((2 * i - 1) % L::stages));
+                                tc_commit(b_empty + 8 * (2 * i % L::stages));
+                            }
                         }
                         __syncwarp();
-                        if (t == 0 && half == 0 && !last) ok = full(2 * i + 2);
+                        if (t + 1 == n_tiles && half == 0 && !last) ok = values_in(i + 1) && (i + 2 == n || full(2 * i + 4));
                     }
                     if (!ok) break;
                     if (!last) scores(t, 2 * i + 2);
                     else if (leader) tc_commit(b_o + 8 * t);
                 }
-                if (ok && leader) {
-                    tc_commit(b_empty + 8 * ((2 * i + 1) % L::stages));
-                    if (!last) tc_commit(b_empty + 8 * ((2 * i + 2) % L::stages));
-                }
                 __syncwarp();
-                if (ok && !last) ok = full(2 * i + 3);
             }
         }
     } else if (!PREFIX && warp == 10 && it.any && p.causal) {
