@@ -22,6 +22,20 @@
 // zero times another sequence's NaN would be NaN).  Values that SOME rows of the CTA see (the causal
 // diagonal) must stay; should one of them be NaN or infinite, warp 10 finds it and the CTA's rows are
 // computed once more row by row (attend_row), where hidden keys are not touched at all.
+//
+// What bounds it (20 heads over 5, 128 channels, one sequence of 8192 tokens, causal: 344 GFLOP): 274 us =
+// 1.25 PFLOP/s, 0.76 of the measured matmul rate; 325 us = 1.06 in runs of seconds, where the board's power
+// cap holds the clock at 1.6 GHz.  A block takes 1.75 us: per tile about 1900 cycles of softmax (80 to load the
+// scores, 380 for the maximum, 700 for each half of the exponentials, which the two warps of a scheduler share)
+// and 1400 until the next scores (the second half of P V, Q K^T, and a few hundred cycles of barriers), while
+// the tensor pipe is busy for 2460 of the 3300.  Weights are handed over in halves, so the product starts on the
+// first while the second is computed (281 us whole).  Tried and slower: 64-key steps with two score buffers (332:
+// Q K^T with 64 columns is bound by shared memory), one product warp per tile (347), the exponentials of the two
+// warps of a scheduler taking turns (+1 %), an eighth to three eighths of the exponentials as a polynomial on
+// the FMA pipe (+1 to +4 %), V and the next K on one barrier (283).  Up to 64 channels the exponentials are
+// the limit (half the products per score); one tile per CTA and two CTAs per SM there: no gain.
+// A CTA's beginning (2.5 us) and end (2.5 us) overlap with nothing: 9 % of the 8192-token prompt, most of a
+// short one.
 #pragma once
 #include "tcgen05.cuh"
 
