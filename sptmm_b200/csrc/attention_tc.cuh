@@ -555,12 +555,12 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
         // ---- loads -------------------------------------------------------------------------------
         bool ok = true;
         const uint32_t group = p.group;
-        if (lane == 0 && n > 0)
-            for (uint32_t t = 0; t < n_tiles; t++) {
-                mbar_expect(b_q + 8 * t, slabs * p.tokens * group * 128);
-                for (uint32_t s = 0; s < slabs; s++)
-                    tma_load_3d(q_smem + t * L::tile + s * 16384, &map_q, b_q + 8 * t, s * 64, kh * group, it.q0 + it.first + t * p.tokens);
-            }
+        auto load_q = [&](uint32_t t) {
+            mbar_expect(b_q + 8 * t, slabs * p.tokens * group * 128);
+            for (uint32_t s = 0; s < slabs; s++)
+                tma_load_3d(q_smem + t * L::tile + s * 16384, &map_q, b_q + 8 * t, s * 64, kh * group, it.q0 + it.first + t * p.tokens);
+        };
+        if (lane == 0 && n > 0) load_q(0);                                          // then K, which tile 0 waits for, then the rest
         if constexpr (PREFIX) {
             // A block is up to eight pages of up to two slabs, a box each: lane s * 8 + g loads slab s of page g,
             // whose number it looked up a block ahead.
@@ -579,6 +579,7 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                 const uint32_t bar = b_full + 8 * st, keys = min(kKeys, p.prefix_len - (it.block0 + i) * kKeys), pages = (keys + size - 1) >> p.page_shift;
                 if (lane == 0) mbar_expect(bar, slabs * pages * size * 128);
                 __syncwarp();
+                if (x == 1 && lane == 0 && n_tiles > 1) load_q(1);
                 if (g < pages && s < slabs) tma_load_4d(ring + st * L::tile + s * 16384 + g * size * 128, x & 1 ? &map_v : &map_k, bar, s * 64, 0, kh, page);
                 if (x & 1) { page = next; next = page_of(i + 2); }
             }
@@ -588,6 +589,7 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                 if (use > 0 && !mbar_wait(b_empty + 8 * st, (use - 1) & 1, abort_word)) { ok = false; break; }
                 issued = x + 1;
                 const uint32_t dst = ring + st * L::tile, bar = b_full + 8 * st, j0 = (it.block0 + i) * kKeys;
+                if (x == 1 && n_tiles > 1) load_q(1);
                 mbar_expect(bar, slabs * 16384);
                 for (uint32_t s = 0; s < slabs; s++) tma_load_3d(dst + s * 16384, x & 1 ? &map_v : &map_k, bar, s * 64, kh, it.k0 + j0);
             }
