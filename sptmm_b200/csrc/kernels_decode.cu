@@ -4,9 +4,9 @@
 // The reference has no attention (its only operator is the matmul, main.cu:993-1961).  HBM bound: a key
 // and its value are read once and used for the query heads that share them.  Three kernels, launched
 // with programmatic overlap:
-//   k_attention_tc<.., true>   (only with a prefix) all rows of the batch against the prefix, each part
-//                              of its keys in another CTA; see attention_tc.cuh
-//   k_decode                   every sequence's own keys
+//   k_attention_tc<.., true>   (only with a prefix and more than 32 rows) all rows of the batch against the
+//                              prefix, each part of its keys in another CTA; see attention_tc.cuh
+//   k_decode                   every sequence's own keys, and the prefix's for few rows
 //   k_decode_join              the parts of a row -> one softmax: with parts (m_i, l_i, o_i) and M = max m_i,
 //                              O = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i
 // k_decode splits the work by keys, not by sequences: all (sequence, key head) units are laid end to end
@@ -42,10 +42,15 @@ struct DecodeParams {
     uint64_t ldq, ldo;
     uint32_t B, heads, group, max_pages, row_tiles, rows;      // rows: query heads per unit, at most 16
     uint32_t partial;                        // never store to O: the prefix's parts are still to be joined
+    uint32_t beside;                         // the prefix's kernel runs before this one
+    // A prefix read by this kernel: `prefix_tiles` tiles of up to 16 of the batch's rows per key head; 0: none
+    const int32_t *prefix_table;
+    uint32_t prefix_len, prefix_tiles;
+    uint32_t piece_rows;                     // rows between pieces
     float scale;                             // scale * log2(e)
     uint2 *span;                             // [unit]: its first and last piece
-    float2 *part_ml;                         // [piece][rows]: (m in powers of two, l)
-    float *part_o;                           // [piece][rows][head_dim]
+    float2 *part_ml;                         // [piece][piece_rows]: (m in powers of two, l)
+    float *part_o;                           // [piece][piece_rows][head_dim]
     // the prefix's parts
     const float2 *prefix_ml;
     const float *prefix_o;
@@ -91,27 +96,33 @@ template <int DP> struct DecodeLayout {
     static constexpr uint32_t smem = ring + kDecodeWarps * 8 * DP * 4;                      // and eight rows of every warp's sums
 };
 
-// A run of blocks of one unit that a CTA takes on.
+// A run of blocks of one unit that a CTA takes on.  b = kPrefix: a tile of the batch's rows over the prefix.
+constexpr uint32_t kPrefix = 0xffffffffu;
 struct Piece {
-    uint32_t b, kh, rt, unit, len, blk0, blk1, blocks;       // blocks: of the whole unit; blk0 .. blk1: this piece
+    uint32_t b, kh, rt, rows, unit, len, blk0, blk1, blocks;       // blocks: of the whole unit; blk0 .. blk1: this piece
 };
 
-// The CTA's way through its run [w, w1) of the units laid end to end.  A unit counts kUnitCost blocks more than
-// it has, the time its first loads and its end take, so that a CTA with many short units gets fewer blocks.
+// The CTA's way through its run [w, w1) of the units laid end to end: the prefix's, if it is read here, then the
+// sequences' one after the other.  A unit counts kUnitCost blocks more than it has, the time its first loads and
+// its end take, so that a CTA with many short units gets fewer blocks.
 constexpr uint32_t kUnitCost = 2;
 struct Walk {
     uint64_t w, w1, at;                      // at: where sequence b begins
-    uint32_t b;
-    __device__ __forceinline__ bool next(const DecodeParams &p, uint32_t per_seq, Piece &x)
+    uint32_t b;                              // kPrefix, 0, 1, ...
+    __device__ __forceinline__ bool next(const DecodeParams &p, Piece &x)
     {
         while (w < w1) {
-            const uint32_t len = own_keys(p, b), nb = (len + kBlockKeys - 1) / kBlockKeys, cost = nb + kUnitCost;
+            const bool pre = b == kPrefix;
+            const uint32_t tiles = pre ? p.prefix_tiles : p.row_tiles, per_seq = p.cache.kv_heads * tiles;
+            const uint32_t len = pre ? p.prefix_len : own_keys(p, b), nb = (len + kBlockKeys - 1) / kBlockKeys, cost = nb + kUnitCost;
             if (nb == 0 || w >= at + (uint64_t)cost * per_seq) { at += nb ? (uint64_t)cost * per_seq : 0; b++; continue; }
             const uint32_t sub = (uint32_t)((w - at) / cost), v0 = (uint32_t)(w - at - (uint64_t)sub * cost), v1 = (uint32_t)min((uint64_t)cost, v0 + (w1 - w));
             w += v1 - v0;
             x.blk0 = v0 > kUnitCost ? v0 - kUnitCost : 0; x.blk1 = v1 > kUnitCost ? v1 - kUnitCost : 0;
             if (x.blk0 == x.blk1) continue;  // only a part of the cost, none of the blocks
-            x.b = b; x.kh = sub / p.row_tiles; x.rt = sub % p.row_tiles; x.unit = b * per_seq + sub; x.len = len; x.blocks = nb;
+            x.b = b; x.kh = sub / tiles; x.rt = sub % tiles; x.len = len; x.blocks = nb;
+            x.rows = min(16u, (pre ? p.B * p.group : p.group) - x.rt * 16);
+            x.unit = (pre ? 0 : p.cache.kv_heads * p.prefix_tiles + b * per_seq) + sub;
             return true;
         }
         x.blk0 = x.blk1 = 0;
@@ -136,8 +147,8 @@ k_decode(const DecodeParams p)
     // Behind the prefix's kernel this one starts when all that came before has ended (that kernel lets it go only
     // then) and reads nothing of the prefix's: it runs beside it, and waits at its own end so that the joining
     // kernel, which waits for this one, finds both done.
-    auto end = [&]() { if (p.partial) pdl_wait_prior_grid(); };
-    if (!p.partial) pdl_wait_prior_grid();
+    auto end = [&]() { if (p.beside) pdl_wait_prior_grid(); };
+    if (!p.beside) pdl_wait_prior_grid();
     // ---- this CTA's run: thread t sums a contiguous range of sequences ---------------------------------
     auto cost_of = [&](uint32_t b) -> uint64_t {
         const uint32_t nb = (own_keys(p, b) + kBlockKeys - 1) / kBlockKeys;
@@ -154,7 +165,8 @@ k_decode(const DecodeParams p)
     }
     if (lane == 31) warp_sum[warp] = upto;
     __syncthreads();
-    uint64_t total = 0, before = upto - mine;
+    const uint64_t prefix_cost = p.prefix_tiles ? (uint64_t)((p.prefix_len + kBlockKeys - 1) / kBlockKeys + kUnitCost) * p.cache.kv_heads * p.prefix_tiles : 0;
+    uint64_t total = prefix_cost, before = prefix_cost + upto - mine;
     for (uint32_t w = 0; w < kDecodeWarps; w++) {
         if (w < warp) before += warp_sum[w];
         total += warp_sum[w];
@@ -168,6 +180,7 @@ k_decode(const DecodeParams p)
     auto start_of = [&](uint64_t c) { return even * c / active + (late ? min(c, (uint64_t)p.early) * p.lead : 0); };
     Walk walk;
     walk.w = start_of(cta); walk.w1 = start_of(cta + 1);
+    if (tid == 0 && walk.w < prefix_cost) { start_b = kPrefix; start_w = 0; }
     if (before <= walk.w && walk.w < before + mine) {
         uint64_t at = before;
         uint32_t b = b_lo;
@@ -182,18 +195,19 @@ k_decode(const DecodeParams p)
     walk.b = start_b; walk.at = start_w;
 
     Piece cur, nxt, iss;                     // worked on, after it, being requested (one of the two)
-    if (!walk.next(p, per_seq, cur)) { end(); return; }
+    if (!walk.next(p, cur)) { end(); return; }
     const uint32_t ring = smem_addr(dyn) + warp * kDecodeStages * L::stage;
     float *sums = reinterpret_cast<float *>(dyn + L::ring);
     // tile i of a piece, for this warp: keys from ((blk0 + i) * warps + warp) * 16
     auto key_of = [&](const Piece &x, uint32_t i) { return ((x.blk0 + i) * kDecodeWarps + warp) * kTileKeys; };
     auto page_of = [&](const Piece &x, uint32_t i) -> uint32_t {
         const uint32_t key = key_of(x, i);
-        return i < x.blk1 - x.blk0 && key < x.len ? (uint32_t)p.table[(uint64_t)x.b * p.max_pages + (key >> p.cache.page_shift)] : 0xffffffffu;
+        if (i >= x.blk1 - x.blk0 || key >= x.len) return 0xffffffffu;
+        return (uint32_t)(x.b == kPrefix ? p.prefix_table : p.table + (uint64_t)x.b * p.max_pages)[key >> p.cache.page_shift];
     };
     uint32_t ii = 0, page_lane = page_of(cur, lane), page_next = page_of(cur, 32 + lane);      // pages of tiles ii & ~31 .. + 32 of `iss`, one per lane; the 32 after
     iss = cur;
-    walk.next(p, per_seq, nxt);
+    walk.next(p, nxt);
     uint32_t nxt_page = page_of(nxt, lane);
     bool on_next = false;                    // iss is nxt
     uint32_t ahead = 0, slot_in = 0, slot_out = 0, valid_bits = 0;      // tiles requested and not used; bit s: the tile in ring slot s lies in the cache
@@ -228,14 +242,19 @@ k_decode(const DecodeParams p)
     request();
     uint32_t qa[DP / 16][4];                 // query rows as A fragments: rows lane / 4 and + 8, channels 2 (lane % 4) and + 8 of every sixteen
     auto load_q = [&](const Piece &x) {
-        const uint32_t rows = min(p.rows, p.group - x.rt * 16);
-        const T *q = static_cast<const T *>(p.Q) + (uint64_t)x.b * p.ldq + (uint64_t)(x.kh * p.group + x.rt * 16) * D;
+        const T *q[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t r = x.rt * 16 + lane / 4 + h * 8;                         // of the group, or of the batch's rows
+            const uint32_t b = x.b == kPrefix ? r / p.group : x.b, g = x.b == kPrefix ? r % p.group : r;
+            q[h] = lane / 4 + h * 8 < x.rows ? static_cast<const T *>(p.Q) + (uint64_t)b * p.ldq + (uint64_t)(x.kh * p.group + g) * D : nullptr;
+        }
 #pragma unroll
         for (int k = 0; k < DP / 16; k++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const uint32_t r = lane / 4 + (e & 1) * 8, c = k * 16 + (lane & 3) * 2 + (e >> 1) * 8;
-                qa[k][e] = r < rows && c < D ? *reinterpret_cast<const uint32_t *>(q + (uint64_t)r * D + c) : 0u;
+                const uint32_t c = k * 16 + (lane & 3) * 2 + (e >> 1) * 8;
+                qa[k][e] = q[e & 1] && c < D ? *reinterpret_cast<const uint32_t *>(q[e & 1] + c) : 0u;
             }
     };
     load_q(cur);
@@ -320,13 +339,13 @@ k_decode(const DecodeParams p)
             if (!on_next) { iss = nxt; ii = 0; page_lane = nxt_page; page_next = page_of(iss, 32 + lane); }
             on_next = false;
             cur = nxt;
-            walk.next(p, per_seq, nxt);
+            walk.next(p, nxt);
             nxt_page = page_of(nxt, lane);
             request();
             load_q(cur);
         }
         // ---- the warps' parts -> one, eight rows at a time -------------------------------------------
-        const uint32_t head0 = done.kh * p.group + done.rt * 16, rows = min(p.rows, p.group - done.rt * 16), piece = done.unit + cta;
+        const uint32_t head0 = done.kh * p.group + done.rt * 16, rows = done.rows, piece = done.unit + cta;
         const bool whole = done.blk0 == 0 && done.blk1 == done.blocks && !p.partial;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -364,8 +383,8 @@ k_decode(const DecodeParams p)
                     *reinterpret_cast<uint2 *>(static_cast<T *>(p.O) + (uint64_t)done.b * p.ldo + (uint64_t)(head0 + row) * D + c) =
                         make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
                 } else {
-                    *reinterpret_cast<float4 *>(p.part_o + ((uint64_t)piece * p.rows + row) * D + c) = v;
-                    if (c == 0) p.part_ml[(uint64_t)piece * p.rows + row] = make_float2(M, sum);
+                    *reinterpret_cast<float4 *>(p.part_o + ((uint64_t)piece * p.piece_rows + row) * D + c) = v;
+                    if (c == 0) p.part_ml[(uint64_t)piece * p.piece_rows + row] = make_float2(M, sum);
                 }
             }
         }
@@ -387,17 +406,22 @@ __global__ void __launch_bounds__(128) k_decode_join(const DecodeParams p)
     __shared__ float4 sums[4][32];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane * 4, D = p.cache.head_dim;
     const uint32_t b = blockIdx.x / p.heads, h = blockIdx.x % p.heads, kh = h / p.group, g = h % p.group;
-    const uint32_t unit = (b * p.cache.kv_heads + kh) * p.row_tiles + g / 16, r = g % 16;
+    const uint32_t unit = p.cache.kv_heads * p.prefix_tiles + (b * p.cache.kv_heads + kh) * p.row_tiles + g / 16, r = g % 16;
+    const uint32_t R = b * p.group + g;      // among the batch's rows, of the prefix read by k_decode
     const uint64_t row = blockIdx.x;
     pdl_launch_dependents();
     pdl_wait_prior_grid();
-    uint32_t first = 0, count = 0;
+    uint32_t first = 0, count = 0, pre_first = 0, pre_count = p.splits;
     const uint2 span = p.span[unit];         // not written where there are no keys: looked at below
     if (own_keys(p, b) > 0) {
         if (span.x == 0xffffffffu) return;   // the whole unit went straight to O
         first = span.x; count = span.y - span.x + 1;
     }
-    const uint32_t parts = p.splits + count, each = (parts + 3) / 4, i0 = min(parts, warp * each), i1 = min(parts, i0 + each);
+    if (p.prefix_tiles) {
+        const uint2 pre = p.span[kh * p.prefix_tiles + R / 16];
+        pre_first = pre.x; pre_count = pre.y - pre.x + 1;
+    }
+    const uint32_t parts = pre_count + count, each = (parts + 3) / 4, i0 = min(parts, warp * each), i1 = min(parts, i0 + each);
     float M = -INFINITY, l = 0;
     float4 o = make_float4(0, 0, 0, 0);
     for (uint32_t i = i0; i < i1; i += 8) {
@@ -408,9 +432,12 @@ __global__ void __launch_bounds__(128) k_decode_join(const DecodeParams p)
             y[k] = make_float2(-INFINITY, 0.0f); v[k] = make_float4(0, 0, 0, 0);
             if (i + k < i1) {
                 const uint32_t part = i + k;
-                const uint64_t at = part < p.splits ? row * p.splits + part : (uint64_t)(first + part - p.splits) * p.rows + r;
-                y[k] = part < p.splits ? p.prefix_ml[at] : p.part_ml[at];
-                if (c < D) v[k] = *reinterpret_cast<const float4 *>((part < p.splits ? p.prefix_o : p.part_o) + at * D + c);
+                const bool split = part < p.splits;              // written by the prefix's kernel; else a piece
+                const uint64_t at = split ? row * p.splits + part
+                                          : part < pre_count ? (uint64_t)(pre_first + part) * p.piece_rows + R % 16
+                                                             : (uint64_t)(first + part - pre_count) * p.piece_rows + r;
+                y[k] = split ? p.prefix_ml[at] : p.part_ml[at];
+                if (c < D) v[k] = *reinterpret_cast<const float4 *>((split ? p.prefix_o : p.part_o) + at * D + c);
             }
         }
         float m1 = M;
@@ -461,19 +488,31 @@ static PrefixPlan plan_prefix(uint32_t B, uint32_t kv_heads, uint32_t group, uin
     return pl;
 }
 
-struct WorkspacePlan { uint64_t span, part_ml, part_o, prefix_ml, prefix_o, bytes; uint32_t row_tiles, rows; PrefixPlan prefix; };
+// Up to this many rows (sequences times query heads per key head) a prefix is read by k_decode itself, a tile of 16
+// rows as if it were one more sequence: no kernel of its own, no tile of 128 rows to fill.  Measured, own kernel
+// against read here: 4 rows over 8192 keys of five key heads 21.1 / 11.8 us, 16 rows 21.5 / 14.0, 32 rows over
+// 16384 keys of eight 47.4 / 26.8; 40 rows 35.3 / 33.1; 64 rows 22.1 / 23.1, 128 rows 22.2 / 31.6.
+constexpr uint64_t kPrefixRows = 32;
+struct WorkspacePlan {
+    uint64_t span, part_ml, part_o, prefix_ml, prefix_o, bytes, units;
+    uint32_t row_tiles, rows, prefix_tiles, piece_rows;
+    PrefixPlan prefix;                       // splits 0: no kernel for the prefix
+};
 static WorkspacePlan plan_workspace(uint32_t B, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t prefix_len)
 {
     WorkspacePlan w{};
     const uint32_t group = heads / kv_heads;
     w.row_tiles = (group + 15) / 16; w.rows = group < 16 ? group : 16;
-    w.prefix = plan_prefix(B, kv_heads, group, prefix_len);
-    const uint64_t units = (uint64_t)B * kv_heads * w.row_tiles, pieces = units + kMaxDecodeCtas, parts = (uint64_t)B * heads * w.prefix.splits;
+    if (prefix_len && (uint64_t)B * group <= kPrefixRows) w.prefix_tiles = (B * group + 15) / 16;
+    else w.prefix = plan_prefix(B, kv_heads, group, prefix_len);
+    w.piece_rows = w.prefix_tiles ? 16 : w.rows;
+    w.units = (uint64_t)B * kv_heads * w.row_tiles + (uint64_t)kv_heads * w.prefix_tiles;
+    const uint64_t pieces = w.units + kMaxDecodeCtas, parts = (uint64_t)B * heads * w.prefix.splits;
     uint64_t cur = 0;
     auto take = [&](uint64_t bytes) { const uint64_t at = cur; cur += (bytes + 255) & ~255ull; return at; };
-    w.span = take(units * sizeof(uint2));
-    w.part_ml = take(pieces * w.rows * sizeof(float2));
-    w.part_o = take(pieces * w.rows * head_dim * sizeof(float));
+    w.span = take(w.units * sizeof(uint2));
+    w.part_ml = take(pieces * w.piece_rows * sizeof(float2));
+    w.part_o = take(pieces * w.piece_rows * head_dim * sizeof(float));
     w.prefix_ml = take(parts * sizeof(float2));
     w.prefix_o = take(parts * head_dim * sizeof(float));
     w.bytes = cur;
@@ -538,13 +577,14 @@ extern "C" int sptmm_attention_decode(const sptmm_decode_params *a, uint32_t fla
         return fail(SPTMM_ERR_INVALID, "%s: workspace of %llu bytes, %llu needed", who, (unsigned long long)(a->workspace ? a->workspace_bytes : 0), (unsigned long long)need);
     const uint32_t kv_heads = a->cache->kv_heads, D = a->cache->head_dim, group = a->heads / kv_heads, dtype = a->cache->dtype;
     const WorkspacePlan w = plan_workspace(a->B, a->heads, kv_heads, D, a->prefix_len);
-    if ((uint64_t)a->B * kv_heads * w.row_tiles + kMaxDecodeCtas > 0x7fffffffull || (uint64_t)w.prefix.pairs * kv_heads * w.prefix.splits > 0x7fffffffull ||
+    if (w.units + kMaxDecodeCtas > 0x7fffffffull || (uint64_t)w.prefix.pairs * kv_heads * w.prefix.splits > 0x7fffffffull ||
         (uint64_t)a->B * a->heads > 0x7fffffffull)
         return fail(SPTMM_ERR_UNSUPPORTED, "%s: %u sequences of %u key heads in one call", who, a->B, kv_heads);
     char *ws = static_cast<char *>(a->workspace);
     prm.Q = a->Q; prm.O = a->O; prm.lengths = a->lengths; prm.table = a->table;
     prm.B = a->B; prm.heads = a->heads; prm.group = group; prm.max_pages = a->max_pages;
-    prm.row_tiles = w.row_tiles; prm.rows = w.rows; prm.partial = a->prefix_len ? 1 : 0;
+    prm.row_tiles = w.row_tiles; prm.rows = w.rows; prm.piece_rows = w.piece_rows; prm.partial = a->prefix_len ? 1 : 0;
+    prm.beside = w.prefix.splits ? 1 : 0; prm.prefix_table = a->prefix_table; prm.prefix_len = a->prefix_len; prm.prefix_tiles = w.prefix_tiles;
     prm.scale = (a->scale > 0.0f ? a->scale : 1.0f / sqrtf((float)D)) * 1.4426950408889634f;      // log2(e): the kernels work with exp2
     prm.span = reinterpret_cast<uint2 *>(ws + w.span);
     prm.part_ml = reinterpret_cast<float2 *>(ws + w.part_ml); prm.part_o = reinterpret_cast<float *>(ws + w.part_o);
@@ -552,7 +592,7 @@ extern "C" int sptmm_attention_decode(const sptmm_decode_params *a, uint32_t fla
     prm.splits = w.prefix.splits;
     TcParams t{};
     CUtensorMap maps[3];
-    if (a->prefix_len) {
+    if (w.prefix.splits) {
         t.Q = a->Q; t.ldq = prm.ldq; t.T = a->B; t.heads = a->heads; t.kv_heads = kv_heads; t.group = group; t.head_dim = D;
         t.tokens = 128 / group; t.group_mul = 65535 / group + 1; t.scale = prm.scale;
         t.prefix_table = a->prefix_table; t.prefix_len = a->prefix_len; t.n_pages = prm.cache.n_pages; t.page_shift = prm.cache.page_shift;
@@ -573,7 +613,7 @@ extern "C" int sptmm_attention_decode(const sptmm_decode_params *a, uint32_t fla
     SPTMM_CUDA_TRY(cudaGetDevice(&dev));
     SPTMM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     const uint32_t ctas = 2 * (uint32_t)sms < kMaxDecodeCtas ? 2 * (uint32_t)sms : kMaxDecodeCtas;
-    if (a->prefix_len) {
+    if (w.prefix.splits) {
         const uint32_t busy = w.prefix.pairs * kv_heads * w.prefix.splits, per_split = (a->prefix_len + kKeys * w.prefix.splits - 1) / (kKeys * w.prefix.splits);
         if (busy < (uint32_t)sms) {
             prm.early = 2 * ((uint32_t)sms - busy) < ctas ? 2 * ((uint32_t)sms - busy) : ctas;

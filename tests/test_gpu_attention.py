@@ -470,6 +470,32 @@ def test_decode(lengths, prefix, H, Hk, D, page, dtype):
 
 
 @TYPES
+@pytest.mark.parametrize("B,own,prefix,H,Hk,D,page", [
+    (1, [5], 1000, 16, 1, 128, 16),                              # one tile of 16 rows
+    (17, [0, 20, 70], 130, 1, 1, 64, 32),                        # seventeen rows: two tiles
+    (8, [33], 700, 8, 2, 128, 64),                               # 32 rows
+    (33, [0, 1, 40], 300, 2, 2, 64, 32),                         # more rows: the prefix's own kernel
+    (16, [33], 700, 8, 2, 128, 64),
+    (33, [7, 0], 129, 4, 2, 64, 64),
+    (70, [3], 1, 4, 4, 8, 128),
+    (20, [100, 2], 4000, 28, 4, 128, 16),
+    (40, [1, 30], 900, 6, 2, 72, 128),
+    (5, [64], 640, 64, 2, 128, 64),
+])
+def test_decode_prefix_for_few_and_many_rows(B, own, prefix, H, Hk, D, page, dtype):
+    b = Batch([own[i % len(own)] for i in range(B)], prefix, H, Hk, D, dtype, page)
+    b.call()
+    b.verify()
+    if prefix > 2 * page:                                        # pages outside the cache, in the middle and at the end
+        drop = [b.prefix_pages[1], b.prefix_pages[-1]]
+        t = b.prefix_table.cpu()
+        t[1], t[-1] = -1, b.n_pages
+        b.prefix_table = t.cuda()
+        b.call()
+        b.verify(drop)
+
+
+@TYPES
 def test_decode_joint_pages_query_stride_and_scale(dtype):
     b = Batch([100, 17, 260], 90, 8, 2, 128, dtype, 32, joint=True, ldq=8 * 128 + 64)
     b.scale = 0.21
