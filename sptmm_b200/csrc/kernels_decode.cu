@@ -40,7 +40,7 @@ struct DecodeParams {
     CacheView cache;
     const int32_t *lengths, *table;
     uint64_t ldq, ldo;
-    uint32_t B, heads, group, max_pages, row_tiles, rows;      // rows: query heads per unit, at most 16
+    uint32_t B, heads, group, max_pages, row_tiles;            // row_tiles: tiles of 16 query heads per key head
     uint32_t partial;                        // never store to O: the prefix's parts are still to be joined
     uint32_t beside;                         // the prefix's kernel runs before this one
     // A prefix read by this kernel: `prefix_tiles` tiles of up to 16 of the batch's rows per key head; 0: none
@@ -495,17 +495,17 @@ static PrefixPlan plan_prefix(uint32_t B, uint32_t kv_heads, uint32_t group, uin
 constexpr uint64_t kPrefixRows = 32;
 struct WorkspacePlan {
     uint64_t span, part_ml, part_o, prefix_ml, prefix_o, bytes, units;
-    uint32_t row_tiles, rows, prefix_tiles, piece_rows;
+    uint32_t row_tiles, prefix_tiles, piece_rows;
     PrefixPlan prefix;                       // splits 0: no kernel for the prefix
 };
 static WorkspacePlan plan_workspace(uint32_t B, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t prefix_len)
 {
     WorkspacePlan w{};
     const uint32_t group = heads / kv_heads;
-    w.row_tiles = (group + 15) / 16; w.rows = group < 16 ? group : 16;
+    w.row_tiles = (group + 15) / 16;
     if (prefix_len && (uint64_t)B * group <= kPrefixRows) w.prefix_tiles = (B * group + 15) / 16;
     else w.prefix = plan_prefix(B, kv_heads, group, prefix_len);
-    w.piece_rows = w.prefix_tiles ? 16 : w.rows;
+    w.piece_rows = w.prefix_tiles || group > 16 ? 16 : group;
     w.units = (uint64_t)B * kv_heads * w.row_tiles + (uint64_t)kv_heads * w.prefix_tiles;
     const uint64_t pieces = w.units + kMaxDecodeCtas, parts = (uint64_t)B * heads * w.prefix.splits;
     uint64_t cur = 0;
@@ -583,7 +583,7 @@ extern "C" int sptmm_attention_decode(const sptmm_decode_params *a, uint32_t fla
     char *ws = static_cast<char *>(a->workspace);
     prm.Q = a->Q; prm.O = a->O; prm.lengths = a->lengths; prm.table = a->table;
     prm.B = a->B; prm.heads = a->heads; prm.group = group; prm.max_pages = a->max_pages;
-    prm.row_tiles = w.row_tiles; prm.rows = w.rows; prm.piece_rows = w.piece_rows; prm.partial = a->prefix_len ? 1 : 0;
+    prm.row_tiles = w.row_tiles; prm.piece_rows = w.piece_rows; prm.partial = a->prefix_len ? 1 : 0;
     prm.beside = w.prefix.splits ? 1 : 0; prm.prefix_table = a->prefix_table; prm.prefix_len = a->prefix_len; prm.prefix_tiles = w.prefix_tiles;
     prm.scale = (a->scale > 0.0f ? a->scale : 1.0f / sqrtf((float)D)) * 1.4426950408889634f;      // log2(e): the kernels work with exp2
     prm.span = reinterpret_cast<uint2 *>(ws + w.span);

@@ -36,9 +36,9 @@ __device__ __forceinline__ uint64_t nanoseconds()
     return t;
 }
 
-// Every wait is bounded: after two seconds, or this many polls (where a wait of the kernel takes
-// microseconds), the waiter raises the CTA's abort word, which ends all other waits of the CTA at their
-// next look at it.
+// Every wait is bounded: after two seconds (and a thousand polls, in case the GPU was away in between), or
+// this many polls, where a wait of the kernel takes microseconds, the waiter raises the CTA's abort word, which
+// ends all other waits of the CTA at their next look at it.
 constexpr uint32_t kWaitPolls = 1u << 24;
 constexpr uint64_t kWaitNs = 2000000000ull;
 
@@ -49,7 +49,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     for (uint32_t i = 0; i < kWaitPolls; i++) {
         if (mbar_try(bar, parity)) return true;
         if (*abort_word) return false;
-        if (nanoseconds() - start > kWaitNs) break;
+        if (i >= 1000 && nanoseconds() - start > kWaitNs) break;
     }
     *abort_word = 1;
     return false;
