@@ -338,6 +338,31 @@ def test_prompt_many_sequences():
     run_prompt(lengths[:300], rng.integers(0, 9, size=300).tolist(), 2, 1, 64, sp.F16)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_many_sequences_of_many_tiles(causal):
+    """More sequences than a warp has lanes, of zero to seven tiles, some with context: every row is written, and
+    the first and last sequences, the longest and one with context are right."""
+    rng = np.random.default_rng(7)
+    lengths = rng.integers(0, 600, size=75).tolist()
+    lengths[3], lengths[40], lengths[74] = 0, 700, 130
+    context = [int(c) for c in rng.integers(0, 900, size=75) * (rng.random(75) < 0.3)]
+    context[74] = 300
+    H, Hk, D = 3, 3, 64
+    qo, ko = offsets(lengths), offsets([n + c for n, c in zip(lengths, context)])
+    q, k, v = randn(1, qo[-1], H, D, scale=1.5), randn(2, ko[-1], Hk, D), randn(3, ko[-1], Hk, D)
+    out = torch.full_like(q, 11.0)
+    sp.attention_prompt(q, k, v, out, i32(qo), i32(ko), 75, qo[-1], ko[-1], H, Hk, D, causal=causal)
+    torch.cuda.synchronize()
+    assert (out != 11).any(-1).all()
+    for s in (0, 31, 32, 40, 74):
+        rows = sorted({0, lengths[s] // 3, lengths[s] - 1}) if lengths[s] else []
+        for i in rows:
+            m = lengths[s] + context[s]
+            top = context[s] + i + 1 if causal else m
+            a, c = qo[s] + i, ko[s]
+            check(out[a:a + 1], *attend(q[a:a + 1], k[c:c + top], v[c:c + top], sp.F16, D ** -0.5, False))
+
+
 def test_prompt_side_stream_repeat_and_graph():
     """Same bits on another stream, from call to call and from a graph; a replay follows new offsets."""
     H, Hk, D, dtype = 8, 2, 128, sp.BF16
