@@ -478,7 +478,8 @@ int sptmm_splitk_free(sptmm_splitk *s);
  * Common rules
  *  - `dtype` is SPTMM_F16 or SPTMM_BF16, the type of Q, K, V, O and the cache.  Scores, softmax
  *    statistics, norms and sums are fp32; a softmax weight is rounded to `dtype` before it multiplies
- *    a value, an output once at the end.
+ *    a value (fp16: to full precision down to 2^-23 of the row's largest weight, then in steps of 2^-33
+ *    of it), an output once at the end.
  *  - `heads` query heads share `kv_heads` key and value heads: head h reads key head
  *    h / (heads / kv_heads); heads is a multiple of kv_heads, at most 128 times it, and below 65536.
  *  - head_dim is a multiple of 8 up to 128.  A row of Q holds its heads back to back (head h at

@@ -14,9 +14,8 @@
 // ring), 9 issues the products, 10 looks for values that are not finite (below).  The products of one
 // tile run while the other tile is in its softmax; tensor memory is full: S0 S1 O0 O1 are 512 columns
 // at 128 channels.
-// When a row's maximum grows, O and l would have to be scaled down; that is put off until it has grown
-// by more than 2^8 (weights then stay below 2^8, harmless in fp32 sums and 16-bit weights alike, whose
-// relative rounding is the same), so after the first blocks it hardly ever happens.
+// When a row's maximum grows, O and l would have to be scaled down; that is put off until it has grown by more
+// than 2^8 (fp16: 2^6; see WeightRange), so after the first blocks it hardly ever happens.
 // Masks: keys a row does not see get the score -inf before the maximum, blocks nobody sees are not
 // visited, values behind the last visible key are overwritten with zeros in shared memory (a weight of
 // zero times another sequence's NaN would be NaN).  Values that SOME rows of the CTA see (the causal
@@ -56,7 +55,7 @@ struct TcParams {
     uint32_t prefix_len, n_pages, page_shift;
     uint32_t splits;                         // CTAs per item, each with an equal part of the keys
     float *part_o;                           // [token][head][split][head_dim], not divided by l
-    float2 *part_ml;                         // [token][head][split]: (m in powers of two, l)
+    float2 *part_ml;                         // [token][head][split]: (m in powers of two, l); l and O 2^up times as large (WeightRange)
     uint32_t *status;
 };
 
@@ -361,8 +360,8 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
 #pragma unroll
                     for (int e = 0; e < 4; e++) mx[e] = max3(mx[e], __uint_as_float(r[c + e]), __uint_as_float(r[c + 4 + e]));
                 const float mb = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                // a first finite maximum, or one more than 2^8 above the one in use: scale O and l
-                const bool grow = mine && mb > m && (m == -INFINITY || (mb - m) * sc > 8.0f);
+                // a first finite maximum, or one too far above the one in use: scale O and l
+                const bool grow = mine && mb > m && (m == -INFINITY || (mb - m) * sc > WeightRange<T>::lag);
                 if (__any_sync(0xffffffffu, grow)) {
                     const float m1 = fmaxf(m, mb), w = m == -INFINITY ? (m1 == -INFINITY ? 1.0f : 0.0f) : ex2((m - m1) * sc);
                     m = m1;
@@ -379,7 +378,7 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                         }
                     }
                 }
-                const float base = m == -INFINITY ? 0.0f : m * sc;
+                const float base = m == -INFINITY ? 0.0f : m * sc - WeightRange<T>::up;
                 const uint64_t sc2 = f2_pack(sc, sc), nb2 = f2_pack(-base, -base);
                 uint64_t sum[2] = {0, 0};
 #pragma unroll

@@ -49,7 +49,7 @@ struct DecodeParams {
     uint32_t piece_rows;                     // rows between pieces
     float scale;                             // scale * log2(e)
     uint2 *span;                             // [unit]: its first and last piece
-    float2 *part_ml;                         // [piece][piece_rows]: (m in powers of two, l)
+    float2 *part_ml;                         // [piece][piece_rows]: (m in powers of two, l); l and O 2^up times as large (WeightRange)
     float *part_o;                           // [piece][piece_rows][head_dim]
     // the prefix's parts
     const float2 *prefix_ml;
@@ -297,8 +297,8 @@ k_decode(const DecodeParams p)
                     mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
                     mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)) * p.scale;
                 }
-                // scale down only when a maximum has grown by more than 2^8 (or is the first)
-                const bool grow = (mx[0] > m[0] && (m[0] == -INFINITY || mx[0] - m[0] > 8.0f)) || (mx[1] > m[1] && (m[1] == -INFINITY || mx[1] - m[1] > 8.0f));
+                // scale down only when a maximum has grown by more than the lag (or is the first)
+                const bool grow = (mx[0] > m[0] && (m[0] == -INFINITY || mx[0] - m[0] > WeightRange<T>::lag)) || (mx[1] > m[1] && (m[1] == -INFINITY || mx[1] - m[1] > WeightRange<T>::lag));
                 if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
@@ -311,7 +311,7 @@ k_decode(const DecodeParams p)
                 uint32_t pa[4];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const float base = m[h] == -INFINITY ? 0.0f : m[h];
+                    const float base = m[h] == -INFINITY ? 0.0f : m[h] - WeightRange<T>::up;
 #pragma unroll
                     for (int n = 0; n < 2; n++) {
                         const float x = ex2(fmaf(s[n][2 * h], p.scale, -base)), y = ex2(fmaf(s[n][2 * h + 1], p.scale, -base));

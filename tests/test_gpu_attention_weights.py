@@ -1,0 +1,98 @@
+"""GPU tests of the attention operators where softmax weights are very unequal, not finite or all zero.
+
+The bound of test_gpu_attention.attend holds where every weight has a type's full precision.  fp16 weights
+are kept as 2^(x - m + 9), m the running maximum and x the score in powers of two (csrc/attention.cuh, WeightRange),
+so one below 2^-14 there is off by at most half of fp16's smallest step, 2^-25.  m is at most the row's true maximum,
+so relative to the largest weight that is at most 2^-25 / 2^9 = 2^-34, and an output may be off by 2^-34 sum |v| / L more,
+with L = sum of 2^(x - largest x), at least 1.  bf16 rounds weights of any size alike.  An fp16 output below 2^-14 is
+off by 2^-25 at most."""
+import pytest
+
+import sptmm_b200 as sp
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from test_gpu_attention import DT, TYPES, Batch, attend, check, i32, offsets, randn      # noqa: E402
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _device():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    torch.cuda.set_device(0)
+    yield
+    torch.cuda.synchronize()
+
+
+def attend_wide(q, k, v, dtype):
+    """attend() of rows that see all keys, with the bound for weights below fp16's full precision."""
+    want, tol = attend(q, k, v, dtype, q.shape[2] ** -0.5, False)
+    if dtype == sp.F16:
+        g = q.shape[1] // k.shape[1]
+        kk, vv = k.double().repeat_interleave(g, 1), v.double().abs().repeat_interleave(g, 1)
+        s = torch.einsum("nhd,mhd->nhm", q.double(), kk) * q.shape[2] ** -0.5
+        L = (s - s.max(-1, keepdim=True).values).exp().sum(-1, keepdim=True)
+        tol = tol + 2.0 ** -34 * vv.sum(0)[None] / L + 2.0 ** -25
+    return want, tol
+
+
+def sink(q, k, v, at, gap, spread):
+    """Key `at` scores `gap` nats above the others, which score about the same (`spread`), and has a value of zero."""
+    D = q.shape[-1]
+    q *= spread
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[at] = 0.0
+    k[at, :, 0] = gap * D ** 0.5 / 8
+    v *= 20.0
+    v += 30.0
+    v[at] = 0.0
+
+
+GAPS = pytest.mark.parametrize("gap,spread", [(10.0, 0.3), (13.0, 0.0), (15.0, 0.3), (17.5, 0.0), (17.5, 0.3)])
+
+
+@TYPES
+@GAPS
+def test_prompt_attention_sink(gap, spread, dtype):
+    """The largest weight's value is zero: the output is carried by thousands of weights far below it."""
+    for H, Hk, D, lengths, context in ((4, 2, 128, [3], [6000]), (4, 4, 64, [2], [6000]), (4, 4, 128, [1] * 40, [1500] * 40), (6, 3, 64, [1] * 60, [900] * 60)):
+        qo, ko = offsets(lengths), offsets([n + c for n, c in zip(lengths, context)])
+        q, k, v = randn(1, qo[-1], H, D, dtype=dtype), randn(2, ko[-1], Hk, D, dtype=dtype), randn(3, ko[-1], Hk, D, dtype=dtype)
+        sink(q, k, v, torch.tensor(ko[:-1], device="cuda") + 5, gap, spread)
+        out = torch.full_like(q, 11.0)
+        sp.attention_prompt(q, k, v, out, i32(qo), i32(ko), len(lengths), qo[-1], ko[-1], H, Hk, D, dtype=dtype)
+        torch.cuda.synchronize()
+        for s in range(0, len(lengths), 13):
+            for i in range(lengths[s]):
+                a, c = qo[s] + i, ko[s]
+                top = context[s] + i + 1
+                check(out[a:a + 1], *attend_wide(q[a:a + 1], k[c:c + top], v[c:c + top], dtype))
+
+
+@TYPES
+@GAPS
+@pytest.mark.parametrize("lengths,prefix,H,Hk,D", [
+    ([6000, 70], 0, 4, 1, 128),
+    ([40, 3], 4000, 8, 2, 128),                                  # the prefix beside the sequences
+    ([40, 3] * 12, 4000, 8, 2, 64),                              # the prefix by its own kernel
+    ([300] * 12, 1500, 8, 2, 128),
+])
+def test_decode_attention_sink(lengths, prefix, H, Hk, D, gap, spread, dtype):
+    b = Batch(lengths, prefix, H, Hk, D, dtype, 16)
+    q, pages = b.q.view(b.B, H, D), [(b.prefix_pages[0] if prefix else rows[0]) for rows in b.rows]
+    flat_k, flat_v = b.k.permute(0, 2, 1, 3), b.v.permute(0, 2, 1, 3)            # [page][slot][head][channel]
+    q *= spread
+    q[..., 0] = 8.0
+    flat_k[..., 0] = 0.0
+    flat_v *= 20.0
+    flat_v += 30.0
+    for p in set(pages):
+        flat_k[p, 5] = 0.0
+        flat_k[p, 5, :, 0] = gap * D ** 0.5 / 8
+        flat_v[p, 5] = 0.0
+    b.call()
+    torch.cuda.synchronize()
+    for i in range(0, b.B, 7):
+        pk, pv = b.keys(b.prefix_pages, prefix)
+        k, v = b.keys(b.rows[i], lengths[i])
+        check(b.out[i:i + 1], *attend_wide(q[i:i + 1], torch.cat((pk, k)), torch.cat((pv, v)), dtype))
