@@ -565,7 +565,8 @@ typedef struct sptmm_decode_params {
     uint32_t B, heads, max_pages, prefix_len;
     float scale;
 } sptmm_decode_params;
-/* 0 on bad arguments.  Grows with B * heads, not with the sequences' lengths. */
+/* Enough for every batch of up to B sequences behind a prefix of up to prefix_len keys (or none) with these
+ * heads.  0 on bad arguments.  Grows with B * heads, not with the sequences' lengths. */
 uint64_t sptmm_attention_decode_workspace(uint32_t B, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t prefix_len);
 int sptmm_attention_decode(const sptmm_decode_params *p, uint32_t flags, void *stream);
 

@@ -539,7 +539,7 @@ def attention_prompt(Q, K, V, out, q_offsets, k_offsets, n_seqs: int, T: int, Tk
 
 
 def attention_decode_workspace(B: int, heads: int, kv_heads: int, head_dim: int, prefix_len: int = 0) -> int:
-    """Bytes of device workspace attention_decode needs."""
+    """Bytes of device workspace attention_decode needs for up to B sequences behind up to prefix_len shared keys."""
     n = int(lib.sptmm_attention_decode_workspace(B, heads, kv_heads, head_dim, prefix_len))
     if n == 0:
         raise ValueError("attention_decode_workspace: " + lib.sptmm_last_error().decode("utf-8", "replace"))

@@ -522,6 +522,25 @@ static WorkspacePlan plan_workspace(uint32_t B, uint32_t heads, uint32_t kv_head
     return w;
 }
 
+// What suffices for every batch of up to B sequences.  The plan of one batch alone may need less than that of a smaller
+// one: a prefix is divided into fewer parts per row as the pairs of tiles get more, and few rows come in pieces of 16.
+// Between two such steps the size grows with B, so the largest is at the end of one or at B; from kPrefixCtas
+// pairs on there is one part per row.
+static uint64_t workspace_bytes_up_to(uint32_t B, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t prefix_len)
+{
+    uint64_t most = plan_workspace(B, heads, kv_heads, head_dim, prefix_len).bytes;
+    if (!prefix_len) return most;
+    auto look = [&](uint64_t b) {
+        if (b >= B) return;
+        const uint64_t bytes = plan_workspace((uint32_t)b, heads, kv_heads, head_dim, prefix_len).bytes;
+        if (bytes > most) most = bytes;
+    };
+    const uint32_t group = heads / kv_heads;
+    look(kPrefixRows / group);               // the last batch whose prefix k_decode reads
+    for (uint64_t pairs = 1; pairs <= kPrefixCtas; pairs++) look(pairs * 2 * (128 / group));
+    return most;
+}
+
 template <typename T, int DP>
 static cudaError_t launch_decode(const DecodeParams &d, const TcParams &t, const PrefixPlan &pl, const CUtensorMap *maps, uint32_t ctas, void *stream, bool pdl)
 {
@@ -549,7 +568,7 @@ extern "C" uint64_t sptmm_attention_decode_workspace(uint32_t B, uint32_t heads,
     const char *who = "attention_decode_workspace";
     if (check_heads(who, heads, kv_heads, head_dim, SPTMM_F16) != SPTMM_OK) return 0;
     if (B > 65536 || prefix_len > 0x7fffffffu - 128) { fail(SPTMM_ERR_INVALID, "%s: B=%u prefix_len=%u", who, B, prefix_len); return 0; }
-    return plan_workspace(B, heads, kv_heads, head_dim, prefix_len).bytes;
+    return workspace_bytes_up_to(B, heads, kv_heads, head_dim, prefix_len);
 }
 
 extern "C" int sptmm_attention_decode(const sptmm_decode_params *a, uint32_t flags, void *stream)
@@ -575,11 +594,10 @@ extern "C" int sptmm_attention_decode(const sptmm_decode_params *a, uint32_t fla
         return fail(SPTMM_ERR_INVALID, "%s: null pointer", who);
     if (!aligned16(a->Q) || !aligned16(a->O) || !aligned16(a->workspace)) return fail(SPTMM_ERR_INVALID, "%s: an address is not 16-byte aligned", who);
     if (!aligned4(a->lengths) || !aligned4(a->table) || !aligned4(a->prefix_table)) return fail(SPTMM_ERR_INVALID, "%s: an index array is not 4-byte aligned", who);
-    const uint64_t need = sptmm_attention_decode_workspace(a->B, a->heads, a->cache->kv_heads, a->cache->head_dim, a->prefix_len);
-    if (!a->workspace || a->workspace_bytes < need)
-        return fail(SPTMM_ERR_INVALID, "%s: workspace of %llu bytes, %llu needed", who, (unsigned long long)(a->workspace ? a->workspace_bytes : 0), (unsigned long long)need);
     const uint32_t kv_heads = a->cache->kv_heads, D = a->cache->head_dim, group = a->heads / kv_heads, dtype = a->cache->dtype;
     const WorkspacePlan w = plan_workspace(a->B, a->heads, kv_heads, D, a->prefix_len);
+    if (!a->workspace || a->workspace_bytes < w.bytes)
+        return fail(SPTMM_ERR_INVALID, "%s: workspace of %llu bytes, %llu needed", who, (unsigned long long)(a->workspace ? a->workspace_bytes : 0), (unsigned long long)w.bytes);
     if (w.units + kMaxDecodeCtas > 0x7fffffffull || (uint64_t)w.prefix.pairs * kv_heads * w.prefix.splits > 0x7fffffffull ||
         (uint64_t)a->B * a->heads > 0x7fffffffull)
         return fail(SPTMM_ERR_UNSUPPORTED, "%s: %u sequences of %u key heads in one call", who, a->B, kv_heads);

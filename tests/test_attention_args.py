@@ -190,3 +190,26 @@ def test_struct_sizes_match_the_header(tmp_path):
         assert int(got[name]) == C.sizeof(cls), name
         for field, _ in cls._fields_:
             assert int(got[name + "." + field]) == getattr(cls, field).offset, (name, field)
+
+
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(20, 5, 128), (8, 2, 128), (16, 16, 64), (8, 1, 128), (128, 1, 64), (100, 4, 96), (2, 1, 8)])
+def test_workspace_suffices_for_smaller_batches_and_prefixes(heads, kv_heads, head_dim):
+    """What is asked for the largest batch and the longest prefix is enough for every smaller one: a call refuses
+    nothing that its own batch does not need."""
+    for prefix in (0, 1, 128, 129, 700, 2048, 8192, 100000):
+        sizes = [sp.attention_decode_workspace(B, heads, kv_heads, head_dim, prefix) for B in range(1, 400)]
+        assert sizes == sorted(sizes), [i + 1 for i in range(1, len(sizes)) if sizes[i] < sizes[i - 1]]
+    for B in (1, 8, 9, 33, 64, 65, 128, 129, 399):
+        sizes = [sp.attention_decode_workspace(B, heads, kv_heads, head_dim, p) for p in (0, 1, 127, 128, 129, 300, 1000, 1900, 5000, 8192, 30000, 1000000)]
+        assert sizes == sorted(sizes), (B, sizes)
+
+
+def test_workspace_of_a_larger_batch_is_taken():
+    """The number of bytes that a call with fewer sequences asks for, as its refusal of 15 bytes names it, is no more
+    than the size for the larger batch."""
+    for big, small, prefix in ((96, 64, 8192), (65, 64, 8192), (129, 128, 8192), (9, 8, 8192), (400, 3, 300)):
+        size = sp.attention_decode_workspace(big, 20, 5, 128, prefix)
+        with pytest.raises(sp.SptmmError) as e:
+            decode(B=small, heads=20, cache=cache(kv_heads=5), prefix_len=prefix, prefix_table=A, workspace_bytes=15)
+        need = int(e.value.message.split(" bytes, ")[1].split()[0])
+        assert need <= size, (big, small, prefix)
