@@ -422,7 +422,9 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                 }
             }
             // the CTAs of the cluster share the rows: first every row's weights, a thread per row, then the rows,
-            // four of a warp at a time from four CTAs at a time (half a warp to a row up to 64 channels)
+            // four of a warp at a time from four CTAs at a time (half a warp to a row up to 64 channels).  A part counts
+            // with a factor of 0 too, so that an infinite value whose weight has underflowed stays seen, as within a part
+            // (one that a row does not see at all is warp 10's business).
             cluster_sync();
             constexpr uint32_t kLanes = DP / 4, kRows = 32 / kLanes, kBatch = 4, kFrom = 4;
             const uint32_t ranks = p.cluster, used = p.tokens * p.group, here = n_here * p.group, weights = q_smem;      // weights: Q is done with; 8 factors and 1 / l per row
@@ -472,7 +474,7 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
                             for (uint32_t b = 0; b < kBatch; b++) {
                                 float f;
                                 asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(weights + (min(x0 + b * 8 * kRows, x_hi - 1) - x_lo) * 32 + (s0 + k) * 4) : "memory");
-                                if (f != 0.0f) { o[b].x += v[k][b].x * f; o[b].y += v[k][b].y * f; o[b].z += v[k][b].z * f; o[b].w += v[k][b].w * f; }
+                                o[b].x += v[k][b].x * f; o[b].y += v[k][b].y * f; o[b].z += v[k][b].z * f; o[b].w += v[k][b].w * f;
                             }
                 }
 #pragma unroll

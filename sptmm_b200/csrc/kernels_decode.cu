@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(128) k_decode_join(const DecodeParams p)
         for (uint32_t k = 0; k < 8; k++) {
             const float f = y[k].x == -INFINITY ? (y[k].y == 0.0f ? 0.0f : 1.0f) : ex2(y[k].x - M);
             l += y[k].y * f;
-            if (f != 0.0f) { o.x += v[k].x * f; o.y += v[k].y * f; o.z += v[k].z * f; o.w += v[k].w * f; }
+            o.x += v[k].x * f; o.y += v[k].y * f; o.z += v[k].z * f; o.w += v[k].w * f;      // a factor of 0 too: an infinite value stays seen
         }
     }
     if (lane == 0) ml[warp] = make_float2(M, l);

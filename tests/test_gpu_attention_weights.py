@@ -96,3 +96,45 @@ def test_decode_attention_sink(lengths, prefix, H, Hk, D, gap, spread, dtype):
         pk, pv = b.keys(b.prefix_pages, prefix)
         k, v = b.keys(b.rows[i], lengths[i])
         check(b.out[i:i + 1], *attend_wide(q[i:i + 1], torch.cat((pk, k)), torch.cat((pv, v)), dtype))
+
+
+def far_value(q, k, v, at, high, value, D):
+    """Key `high` scores 200 nats above the others, whose weights beside it are zero in 32 bits; key `at` has a
+    value that is not finite in channel 3."""
+    q[..., 0], k[..., 0] = 16.0, 0.0
+    k[high][..., 0] = 200 * D ** 0.5 / 16
+    v[at][..., 3] = value
+
+
+@TYPES
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("at,high", [(2, 3), (20, 40), (10, 2900), (2900, 10), (1500, 1400)])
+def test_a_value_that_is_not_finite_is_seen_whatever_its_weight(at, high, value, dtype):
+    """0 times infinity, as in 32 bits: the same wherever the row's keys are divided -- within a tile, between warps,
+    between CTAs and between the prefix and a sequence's own keys."""
+    H, Hk, D, m = 4, 2, 128, 3000
+    for lengths, context in (([2], [m - 2]), ([2] * 40, [m - 2] * 40)):           # clusters share the keys; one CTA has them all
+        qo, ko = offsets(lengths), offsets([n + c for n, c in zip(lengths, context)])
+        q, k, v = randn(1, qo[-1], H, D, dtype=dtype), randn(2, ko[-1], Hk, D, dtype=dtype), randn(3, ko[-1], Hk, D, dtype=dtype)
+        for s in range(len(lengths)):
+            far_value(q[qo[s]:qo[s + 1]], k[ko[s]:ko[s + 1]], v[ko[s]:ko[s + 1]], at, high, value, D)
+        out = torch.full_like(q, 11.0)
+        sp.attention_prompt(q, k, v, out, i32(qo), i32(ko), len(lengths), qo[-1], ko[-1], H, Hk, D, dtype=dtype)
+        torch.cuda.synchronize()
+        assert not torch.isfinite(out[..., 3]).any()
+        out[..., 3] = 0
+        assert torch.isfinite(out).all()
+    for B, prefix in ((1, 0), (5, 1000), (20, 1000)):
+        b = Batch([m - prefix] * B, prefix, H, Hk, D, dtype, 16)
+        for i in range(B):
+            (pa, sa), (ph, sh) = [((b.prefix_pages if j < prefix else b.rows[i])[(j if j < prefix else j - prefix) // 16],
+                                   (j if j < prefix else j - prefix) % 16) for j in (at, high)]
+            if i == 0:
+                b.q.view(B, H, D)[..., 0], b.k[..., 0] = 16.0, 0.0
+            b.k[ph, :, sh, 0] = 200 * D ** 0.5 / 16
+            b.v[pa, :, sa, 3] = value
+        b.call()
+        torch.cuda.synchronize()
+        assert not torch.isfinite(b.out[..., 3]).any(), (B, prefix)
+        b.out[..., 3] = 0
+        assert torch.isfinite(b.out).all()
