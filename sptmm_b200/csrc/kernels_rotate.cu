@@ -55,7 +55,7 @@ template <typename TI, typename TO, int LPH>
 __global__ void __launch_bounds__(kRotateThreads, 5) k_rotate(const __grid_constant__ RotateParams p)
 {
     using Raw = typename In4<TI>::raw;
-    __shared__ float2 turn[kMaxHeadDim / 2];                 // (cos, sin) of the token's angles
+    __shared__ alignas(16) float2 turn[kMaxHeadDim / 2];     // (cos, sin) of the token's angles, read two at a time
     constexpr uint32_t GROUPS = kRotateThreads / LPH;
     const uint32_t tid = threadIdx.x, lane = tid % LPH, group = tid / LPH, mask = ((1u << LPH) - 1) << (tid & 31 & ~(LPH - 1));
     const uint32_t D = p.head_dim, rot = p.rot_dim, qk_heads = p.heads + p.kv_heads, n_heads = qk_heads + p.kv_heads;
