@@ -13,7 +13,7 @@ import sptmm_b200 as sp
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_attention import DT, TYPES, Batch, attend, check, i32, offsets, randn      # noqa: E402
+from test_gpu_attention import NAN, TYPES, Batch, attend, check, i32, offsets, randn      # noqa: E402
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -138,3 +138,31 @@ def test_a_value_that_is_not_finite_is_seen_whatever_its_weight(at, high, value,
         assert not torch.isfinite(b.out[..., 3]).any(), (B, prefix)
         b.out[..., 3] = 0
         assert torch.isfinite(b.out).all()
+
+
+@TYPES
+def test_rows_whose_scores_are_all_minus_infinity_are_zero(dtype):
+    """Wherever the row is computed: by one CTA or several, or by itself because a value behind it is not finite."""
+    ninf = float("-inf")
+    for H, Hk, D, n, m in ((4, 2, 128, 3, 3000), (4, 4, 64, 2, 1500), (4, 2, 128, 40, 90), (2, 1, 64, 300, 300)):
+        q, k, v = torch.zeros((n, H, D)), torch.zeros((m, Hk, D)), randn(3, m, Hk, D, dtype=dtype)
+        q[..., 0], k[..., 0] = 1.0, ninf
+        q, k = q.to(v), k.to(v)
+        for last in (1.0, NAN):
+            v[m - 1] = last
+            out = torch.full_like(q, 11.0)
+            sp.attention_prompt(q, k, v, out, i32([0, n]), i32([0, m]), 1, n, m, H, Hk, D, dtype=dtype)
+            torch.cuda.synchronize()
+            assert (out[:n - 1] == 0).all()
+            assert torch.isnan(out[n - 1]).all() if last != last else (out[n - 1] == 0).all()
+    for lengths, prefix, H, Hk, D in (([300], 0, 4, 2, 128), ([3000, 20], 0, 4, 2, 64), ([5, 70], 400, 8, 2, 128), ([5, 70] * 9, 400, 8, 2, 128)):
+        b = Batch(lengths, prefix, H, Hk, D, dtype, 16)
+        b.q.zero_()
+        b.q.view(b.B, H, D)[..., 0] = 1.0
+        keep = torch.isnan(b.k)
+        b.k.zero_()
+        b.k[..., 0] = ninf
+        b.k[keep] = NAN
+        b.call()
+        torch.cuda.synchronize()
+        assert (b.out == 0).all()
