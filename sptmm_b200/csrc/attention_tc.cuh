@@ -153,79 +153,83 @@ __device__ __forceinline__ void seq_range(const TcParams &p, uint32_t s, uint32_
     q0 = a; n = b - a; k0 = c; m = d - c;
 }
 
-// Items (pairs of tiles) in falling order of the keys they visit, so that the longest start first and
-// the short ones fill the end.  An item's level is the number of its pair of tiles counted from the
-// sequence's first key; rank `w` is looked up by counting the items at or above a level (a warp, lanes
-// over sequences).
-__device__ __forceinline__ bool find_item(const TcParams &p, uint32_t w, uint32_t &seq, uint32_t &pair)
+// Items are pairs of tiles.  Up to kOrderedSeqs sequences they are taken in falling order of the keys they visit, so
+// that the longest start first and the short ones fill the end.  An item's level is the number of its pair of tiles
+// counted from the sequence's first key; rank `w` is looked up by counting the items at or above a level (a warp, a
+// lane per sequence).
+// For more sequences that would cost every CTA a few passes over all of them: 0.4 ms a call for 700 sequences of one
+// token and 54 ms for 8192.  Then items are numbered by the offsets alone, sequence after sequence: those of s begin
+// at q_off[s] / per + s, which leaves room for every partly filled pair and grows with s, so that a search in at most
+// four steps finds s (0.18 and 1.9 ms).  Measured, ordered / by offset (20 heads over 5, lengths spread over their
+// logarithm up to 1024): 16 sequences 31.7 / 32.5 us, 33 38 / 35, 64 96 / 85, 128 231 / 184; up to 4096 and in rising
+// order, the longest last: 33 sequences 153 / 134, 64 476 / 424.
+constexpr uint32_t kOrderedSeqs = 32;
+// How many numbers the items of a call may take.
+inline uint64_t item_numbers(uint64_t n_seqs, uint64_t T, uint64_t per)
+{
+    if (n_seqs > kOrderedSeqs) return T / per + n_seqs;
+    return (T + (n_seqs < T ? n_seqs : T) * (per - 1)) / per;      // every sequence may end with a part of a pair
+}
+
+__device__ __forceinline__ bool find_item_by_offset(const TcParams &p, uint32_t w, uint32_t &seq, uint32_t &pair)
 {
     const uint32_t lane = threadIdx.x & 31, per = 2 * p.tokens;
+    auto begin = [&](uint32_t s) { return (uint32_t)min(max(p.q_off[s], 0), (int32_t)p.T) / per + s; };
+    uint32_t lo = 0, span = p.n_seqs;        // begin(lo) <= w, and the last such sequence is one of lo .. lo + span
+    if (begin(0) > w) return false;
+    while (span > 1) {
+        const uint32_t step = (span + 31) / 32, at = lane * step;
+        const uint32_t last = 31 - __clz(__ballot_sync(0xffffffffu, at < span && begin(lo + at) <= w));      // lane 0 is always among them
+        lo += last * step;
+        span = min(step, span - last * step);
+    }
+    uint32_t q0, nq, k0, m;
+    seq_range(p, lo, q0, nq, k0, m);
+    const uint32_t n = (nq + per - 1) / per, i = w - begin(lo);
+    seq = lo;
+    pair = p.causal ? n - 1 - i : i;
+    return i < n;
+}
+
+__device__ __forceinline__ bool find_item(const TcParams &p, uint32_t w, uint32_t &seq, uint32_t &pair)
+{
+    if (p.n_seqs > kOrderedSeqs) return find_item_by_offset(p, w, seq, pair);
+    const uint32_t lane = threadIdx.x & 31, per = 2 * p.tokens;
+    uint32_t q0, nq, k0, m, n = 0, low = 0;  // items and first level of sequence `lane`
     if (p.n_seqs == 1) {
-        uint32_t q0, nq, k0, m;
         seq_range(p, 0, q0, nq, k0, m);
-        const uint32_t n = (nq + per - 1) / per;
+        n = (nq + per - 1) / per;
         seq = 0;
         pair = p.causal ? n - 1 - w : w;
         return w < n;
     }
-    // items and first level of sequence s
-    auto shape = [&](uint32_t s, uint32_t &n, uint32_t &low) {
-        uint32_t q0, nq, k0, m;
-        seq_range(p, s, q0, nq, k0, m);
+    if (lane < p.n_seqs) {
+        seq_range(p, lane, q0, nq, k0, m);
         n = (nq + per - 1) / per;
         low = p.causal ? (m > nq ? (m - nq) / per : 0u) : m / per;
-    };
-    auto at_or_above = [&](uint32_t n, uint32_t low, uint32_t x) -> uint32_t {
+    }
+    auto at_or_above = [&](uint32_t x) -> uint32_t {
         if (!p.causal) return low >= x ? n : 0u;
         return x <= low ? n : (x - low >= n ? 0u : n - (x - low));
     };
-    uint32_t n1 = 0, low1 = 0;               // the first 32 sequences stay in registers
-    if (lane < p.n_seqs) shape(lane, n1, low1);
-    uint32_t top = n1 + low1, total = n1;
-    for (uint32_t s = lane + 32; s < p.n_seqs; s += 32) {
-        uint32_t n, low;
-        shape(s, n, low);
-        top = max(top, n + low); total += n;
-    }
-    total = __reduce_add_sync(0xffffffffu, total);
-    if (w >= total) return false;
-    auto count = [&](uint32_t x) {
-        uint32_t c = at_or_above(n1, low1, x);
-        for (uint32_t s = lane + 32; s < p.n_seqs; s += 32) {
-            uint32_t n, low;
-            shape(s, n, low);
-            c += at_or_above(n, low, x);
-        }
-        return __reduce_add_sync(0xffffffffu, c);
-    };
-    uint32_t lo = 0, hi = __reduce_max_sync(0xffffffffu, top) + 1;          // count(lo) > w, count(hi) <= w
+    auto count = [&](uint32_t x) { return __reduce_add_sync(0xffffffffu, at_or_above(x)); };
+    if (w >= count(0)) return false;
+    uint32_t lo = 0, hi = __reduce_max_sync(0xffffffffu, n + low) + 1;          // count(lo) > w, count(hi) <= w
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) / 2;
         if (count(mid) > w) lo = mid; else hi = mid;
     }
-    uint32_t left = w - count(lo + 1);       // among the items of level lo, in order of sequences
-    for (uint32_t s0 = 0; s0 < p.n_seqs; s0 += 32) {
-        const uint32_t s = s0 + lane;
-        uint32_t n = n1, low = low1;
-        if (s0) { n = low = 0; if (s < p.n_seqs) shape(s, n, low); }
-        const uint32_t here = at_or_above(n, low, lo) - at_or_above(n, low, lo + 1);
-        uint32_t sum = here;                 // inclusive prefix over the lanes
+    const uint32_t left = w - count(lo + 1), here = at_or_above(lo) - at_or_above(lo + 1);       // among the items of level lo, in order of sequences
+    uint32_t sum = here;                     // inclusive prefix over the lanes
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= (uint32_t)o) sum += y;
-        }
-        const uint32_t hit = __ballot_sync(0xffffffffu, left < sum);
-        if (hit) {
-            const int src = __ffs(hit) - 1;
-            const uint32_t before = sum - here, pr = p.causal ? lo - low : left - before;
-            seq = s0 + src;
-            pair = __shfl_sync(0xffffffffu, pr, src);
-            return true;
-        }
-        left -= __shfl_sync(0xffffffffu, sum, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= (uint32_t)o) sum += y;
     }
-    return false;
+    const int src = __ffs(__ballot_sync(0xffffffffu, left < sum)) - 1;
+    seq = src;
+    pair = __shfl_sync(0xffffffffu, p.causal ? lo - low : left - (sum - here), src);
+    return true;
 }
 
 // SPLIT: clusters share the keys of an item.  A variant of its own, because what it keeps for the end costs the

@@ -88,8 +88,7 @@ extern "C" int sptmm_attention_prompt(const sptmm_prompt_params *a, uint32_t fla
     prm.head_dim = a->head_dim; prm.causal = a->causal ? 1 : 0;
     prm.tokens = 128 / prm.group; prm.group_mul = 65535 / prm.group + 1;
     prm.scale = (a->scale > 0.0f ? a->scale : 1.0f / sqrtf((float)a->head_dim)) * 1.4426950408889634f;     // log2(e): the kernel works with exp2
-    // pairs of tiles: every sequence may end with a part of one
-    const uint64_t per = 2 * prm.tokens, seqs = a->n_seqs < a->T ? a->n_seqs : a->T, items = ((uint64_t)a->T + seqs * (per - 1)) / per;
+    const uint64_t items = item_numbers(a->n_seqs, a->T, 2 * prm.tokens);
     if (items * a->kv_heads > 0x7fffffffull / 8) return fail(SPTMM_ERR_UNSUPPORTED, "%s: %u rows of %u key heads in one call", who, a->T, a->kv_heads);
     // Few items leave SMs idle: then up to eight CTAs, as many as there is an SM for, share an item's keys
     // (if it has two blocks of keys for each; see the kernel).  512 queries over 8192 keys, 40 items: 126 us by
