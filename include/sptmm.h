@@ -576,6 +576,13 @@ int sptmm_attention_decode(const sptmm_decode_params *p, uint32_t flags, void *s
  * those of the matmuls.  Waits for the current device and reads the word a wait that ran out raises
  * there; 0 = every attention call since the last look completed normally. */
 int sptmm_attention_status(uint32_t *status);
+/* A limit on the time of every CTA of the tensor-core attention kernels (prompts, a shared prefix) in this process's
+ * calls from now on (a captured call keeps its own): how often, some tens of nanoseconds apart, it is looked whether
+ * its last product is done before its waits are ended.  0 = none but that of each wait, two seconds where one takes
+ * microseconds.  A call in which a limit ran out ends by itself: the loads and products that it issued are waited
+ * for, rows of O may be missing or wrong, the device and the library stay usable.  A CTA needs 1.75 us for 128
+ * keys and 5 us more; a limit of one look always runs out, which is how that is tested. */
+int sptmm_attention_set_wait_limit(uint32_t polls);
 
 /* ---- small device helpers so a C caller needs no CUDA headers ------------------------------ */
 int sptmm_device_count(int *count);

@@ -120,6 +120,7 @@ def _load() -> C.CDLL:
         "sptmm_attention_decode_workspace": (u64, [u32, u32, u32, u32, u32]),
         "sptmm_attention_decode": (i32, [vp, u32, vp]),
         "sptmm_attention_status": (i32, [C.POINTER(u32)]),
+        "sptmm_attention_set_wait_limit": (i32, [u32]),
         "sptmm_device_count": (i32, [C.POINTER(C.c_int)]),
         "sptmm_set_device": (i32, [C.c_int]),
         "sptmm_dev_alloc": (i32, [C.POINTER(vp), u64]),
@@ -152,7 +153,7 @@ EXPORTS = ["sptmm_last_error", "sptmm_version", "sptmm_gen_ternary_fixed", "sptm
            "sptmm_splitk_clear", "sptmm_splitk_barrier", "sptmm_splitk_accumulate", "sptmm_splitk_output", "sptmm_splitk_status",
            "sptmm_splitk_set_wait_limit", "sptmm_splitk_free",
            "sptmm_rotate_heads", "sptmm_attention_prompt", "sptmm_attention_decode_workspace", "sptmm_attention_decode",
-           "sptmm_attention_status",
+           "sptmm_attention_status", "sptmm_attention_set_wait_limit",
            "sptmm_device_count", "sptmm_set_device", "sptmm_dev_alloc", "sptmm_dev_free",
            "sptmm_memcpy_h2d", "sptmm_memcpy_d2h", "sptmm_device_sync", "sptmm_stream_wait"]
 
@@ -560,6 +561,12 @@ def attention_status() -> int:
     st = C.c_uint32(0)
     check(lib.sptmm_attention_status(C.byref(st)))
     return st.value
+
+
+def attention_set_wait_limit(polls: int) -> None:
+    """How often a CTA of the prompt and prefix kernels looks for the end of its products, in the calls from now on, before
+    its waits are ended (sptmm_attention_set_wait_limit); 0 = no limit but that of each wait, two seconds."""
+    check(lib.sptmm_attention_set_wait_limit(polls))
 
 
 def row_split3_small(X, W_pos_div, W_neg_div, out, M: int, K: int, N: int, S: int, split: int, stream: int = 0) -> None:

@@ -11,7 +11,8 @@
 //     P = 2^(S scale - m)        one thread per row: m, l and the weights need no exchange between lanes
 //     O += P V                   tcgen05, P (16 bit) from tensor memory where S was, O in tensor memory
 // Warps: 0-3 the softmax of tile 0, 4-7 of tile 1, 8 the TMA loads (Q once, K and V blocks through a
-// ring), 9 issues the products, 10 looks for values that are not finite (below).  The products of one
+// ring), 9 issues the products, 10 looks for values that are not finite (below), 11 keeps a caller's limit on the
+// CTA's time, if there is one.  The products of one
 // tile run while the other tile is in its softmax; tensor memory is full: S0 S1 O0 O1 are 512 columns
 // at 128 channels.
 // When a row's maximum grows, O and l would have to be scaled down; that is put off until it has grown by more
@@ -57,6 +58,7 @@ struct TcParams {
     float *part_o;                           // [token][head][split][head_dim], not divided by l
     float2 *part_ml;                         // [token][head][split]: (m in powers of two, l); l and O 2^up times as large (WeightRange)
     uint32_t *status;
+    uint32_t wait_polls;                     // looks at its last product that a CTA may take; 0: no limit but that of every wait
 };
 
 constexpr uint32_t kTcThreads = 384;        // three warpgroups: two of softmax, one of loads, products and the value check
@@ -692,23 +694,27 @@ k_attention_tc(const __grid_constant__ TcParams p, const __grid_constant__ CUten
             }
         }
         if (__any_sync(0xffffffffu, found) && lane == 0) bad_values = 1;
+    } else if (warp == 11 && p.wait_polls && n > 0) {
+        // ---- the caller's limit: ends the waits of the others unless the last product is done by then -----------
+        mbar_poll(b_o + 8 * (n_tiles - 1), 0, abort_word, p.wait_polls);             // (tested in the waits themselves it costs a long prompt 3 %)
     }
     __syncwarp();
     if (SPLIT && warp >= 8 && spread) cluster_sync();         // the one the softmax warps pass before they join
     __syncthreads();
     if (abort_flag) {
-        // a wait ran out (never in a healthy run): report, then let copies and products in flight end
+        // a wait ran out (never in a healthy run with the default limit): report, then let copies and products in flight end
         if (tid == 0) atomicOr(p.status, 1u);
         uint32_t never = 0;
         if (warp == 9 && n > 0) {
             __syncwarp();
             if (elect_one()) tc_commit(b_end);       // arrives when every product issued so far is done
-            mbar_wait(b_end, 0, &never);
+            mbar_wait_warp(b_end, 0, &never);
         }
         if (tid == 8 * 32 && n > 0) {
             for (uint32_t t = 0; t < n_tiles; t++) mbar_wait(b_q + 8 * t, 0, &never);
             for (uint32_t x = issued > L::stages ? issued - L::stages : 0; x < issued; x++) mbar_wait(b_full + 8 * (x % L::stages), x / L::stages & 1, &never);
         }
+        __syncwarp();
         __syncthreads();
     }
     if (SPLIT && spread) cluster_sync();     // nobody leaves while its memory is read

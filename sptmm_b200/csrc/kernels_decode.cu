@@ -621,6 +621,7 @@ extern "C" int sptmm_attention_decode(const sptmm_decode_params *a, uint32_t fla
         t.part_o = reinterpret_cast<float *>(ws + w.prefix_o); t.part_ml = reinterpret_cast<float2 *>(ws + w.prefix_ml);
         rc = attention_status_word(&t.status);
         if (rc != SPTMM_OK) return rc;
+        t.wait_polls = attention_wait_polls();
         const uint64_t dims_q[3] = {D, a->heads, a->B}, str_q[2] = {D * 2ull, prm.ldq * 2};
         const uint64_t dims_k[4] = {D, a->cache->page_size, kv_heads, a->cache->n_pages};
         const uint64_t str_k[3] = {D * 2ull, (uint64_t)a->cache->page_size * D * 2, prm.cache.page_stride * 2};

@@ -17,6 +17,10 @@ int attention_status_word(uint32_t **dev_word)
     return SPTMM_OK;
 }
 
+static std::atomic<uint32_t> g_wait_polls{0};        // 0: the default
+
+uint32_t attention_wait_polls() { return g_wait_polls.load(); }
+
 using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                  const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
@@ -100,6 +104,7 @@ extern "C" int sptmm_attention_prompt(const sptmm_prompt_params *a, uint32_t fla
     prm.cluster = room > 8 ? 8 : room < 1 ? 1 : (uint32_t)room;
     rc = attention_status_word(&prm.status);
     if (rc != SPTMM_OK) return rc;
+    prm.wait_polls = attention_wait_polls();
     const uint64_t D = a->head_dim, es = 2;
     const uint64_t dims_q[3] = {D, a->heads, a->T}, str_q[2] = {D * es, prm.ldq * es};
     const uint64_t dims_k[3] = {D, a->kv_heads, a->Tk ? a->Tk : 1}, str_k[2] = {D * es, prm.ldk * es}, str_v[2] = {D * es, prm.ldv * es};
@@ -113,6 +118,12 @@ extern "C" int sptmm_attention_prompt(const sptmm_prompt_params *a, uint32_t fla
     const bool pdl = flags & SPTMM_LAUNCH_PDL;
     const cudaError_t e = a->dtype == SPTMM_F16 ? launch_prompt<__half>(prm, grid, mq, mk, mv, stream, pdl) : launch_prompt<__nv_bfloat16>(prm, grid, mq, mk, mv, stream, pdl);
     if (e != cudaSuccess) return fail(SPTMM_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+    return SPTMM_OK;
+}
+
+extern "C" int sptmm_attention_set_wait_limit(uint32_t polls)
+{
+    g_wait_polls.store(polls);
     return SPTMM_OK;
 }
 

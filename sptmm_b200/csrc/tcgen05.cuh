@@ -60,6 +60,19 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_word));
 }
 
+// A wait that raises the abort word after `polls` looks, none of which suspends the thread.  Not inlined: the kernel's
+// softmax loop would spill registers for it (a prompt of 8192 tokens 282 us for 276).
+static __device__ __noinline__ void mbar_poll(uint32_t bar, uint32_t parity, volatile uint32_t *abort_word, uint32_t polls)
+{
+    for (uint32_t i = 0; i < polls; i++) {
+        uint32_t ok;
+        asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok || *abort_word) return;
+    }
+    *abort_word = 1;
+}
+
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z)
 {
     asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -205,5 +218,6 @@ __device__ __forceinline__ float max3(float a, float b, float c)
 int make_tensor_map(const char *who, CUtensorMap *map, const void *base, uint32_t dtype, uint32_t rank, const uint64_t *dims,
                     const uint64_t *strides, const uint32_t *box);
 int attention_status_word(uint32_t **dev_word);      // device address of the library's word for expired waits
+uint32_t attention_wait_polls();                     // of the calls from now on; 0: no limit
 
 }  // namespace sptmm
