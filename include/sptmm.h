@@ -492,6 +492,7 @@ int sptmm_splitk_free(sptmm_splitk *s);
  *    rows) is left out, not followed.
  *  - A query without any visible key gives a row of zeros, and so does one whose visible keys all score
  *    -infinity (where their values are finite): nothing is left of the row, as when it is masked.
+ *  - All buffers are the current device's, and so is the stream.
  *  - No call allocates or synchronises; all may be captured into a graph (like every kernel of a library,
  *    theirs are loaded by the first call on a device, which is best made before a capture).
  *    SPTMM_LAUNCH_PDL in `flags` as for the matmuls. */

@@ -23,8 +23,8 @@
 // diagonal) must stay; should one of them be NaN or infinite, warp 10 finds it and the CTA's rows are
 // computed once more row by row (attend_row), where hidden keys are not touched at all.
 //
-// What bounds it (20 heads over 5, 128 channels, one sequence of 8192 tokens, causal: 344 GFLOP): 274 us =
-// 1.25 PFLOP/s, 0.76 of the measured matmul rate; 325 us = 1.06 in runs of seconds, where the board's power
+// What bounds it (20 heads over 5, 128 channels, one sequence of 8192 tokens, causal: 344 GFLOP): 272 to 277 us
+// = 1.25 PFLOP/s, 0.76 of the measured matmul rate; 321 us = 1.07 in runs of seconds, where the board's power
 // cap holds the clock at 1.6 GHz.  A block takes 1.75 us: per tile about 1900 cycles of softmax (80 to load the
 // scores, 380 for the maximum, 700 for each half of the exponentials, which the two warps of a scheduler share)
 // and 1400 until the next scores (the second half of P V, Q K^T, and a few hundred cycles of barriers), while

@@ -96,7 +96,7 @@ extern "C" int sptmm_attention_prompt(const sptmm_prompt_params *a, uint32_t fla
     if (items * a->kv_heads > 0x7fffffffull / 8) return fail(SPTMM_ERR_UNSUPPORTED, "%s: %u rows of %u key heads in one call", who, a->T, a->kv_heads);
     // Few items leave SMs idle: then up to eight CTAs, as many as there is an SM for, share an item's keys
     // (if it has two blocks of keys for each; see the kernel).  512 queries over 8192 keys, 40 items: 126 us by
-    // 40 CTAs, 52 to 58 us by as many clusters of three.
+    // 40 CTAs, 51 to 66 us, from process to process, by as many clusters of three.
     int dev = 0, sms = 0;
     SPTMM_CUDA_TRY(cudaGetDevice(&dev));
     SPTMM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));

@@ -12,7 +12,7 @@
 // all of its heads.  All loads of a token are in flight while the angles are formed:
 // position * inv_freq / 2 pi in 64 bits, reduced to a fraction of a turn, then sincospif in 32 -- at
 // position 131071 a product in 32 bits would already be off by 2^-8 radians.
-// Measured on 8192 tokens of 20 + 5 + 5 heads of 128 channels, fp32 -> bf16 (210 MB): 36 us, 5.8 TB/s, 0.89
+// Measured on 8192 tokens of 20 + 5 + 5 heads of 128 channels, fp32 -> bf16 (210 MB): 36 to 37 us, 5.7 TB/s, 0.87
 // of the copy rate, with five CTAs per SM (48 registers); four or six: 38.6, 36.6; eight (32 registers):
 // 47.9.  Four channels per lane with partners shuffled: 57.  CTAs that walk over tokens and fetch the next
 // one's heads ahead: 64, for the registers that takes.  One to sixteen tokens: 2.9 us, a launch.
