@@ -92,3 +92,46 @@ def test_offsets_that_fall_stay_within_the_buffers():
             sp.attention_prompt(q, k, v, wide, off, off, n_seqs, T, T, H, Hk, D)
             torch.cuda.synchronize()
             assert (wide[T:] == 11).all()
+
+
+def test_no_keys_at_all_and_only_empty_sequences():
+    T, H, Hk, D = 37, 4, 2, 64
+    q, out = randn(1, T, H, D), torch.full((T, H, D), 11.0, dtype=torch.float16, device="cuda")
+    for causal in (True, False):
+        out.fill_(11.0)
+        sp.attention_prompt(q, None, None, out, i32([0, 30, 30, 33]), i32([0, 0, 0, 0]), 3, T, 0, H, Hk, D, causal=causal)
+        torch.cuda.synchronize()
+        assert (out[:33] == 0).all() and (out[33:] == 11).all()
+    out.fill_(11.0)
+    k = randn(2, T, Hk, D)
+    for n in (1, 7, 40):
+        sp.attention_prompt(q, k, k, out, i32([5] * (n + 1)), i32([9] * (n + 1)), n, T, T, H, Hk, D)
+    torch.cuda.synchronize()
+    assert (out == 11).all()
+
+
+def test_rows_beyond_32_bit_offsets():
+    """Q, K, V and O as column ranges of one buffer whose rows lie so far apart that the last ones pass 2^32 elements;
+    a value that is not finite among the last keys, so that the rows that do not see it go one by one."""
+    T, ld, H, Hk, D = 70000, 65536, 2, 1, 128
+    buf = torch.empty((T, ld), dtype=torch.float16, device="cuda")               # 9.2 GB, of which a hundredth is looked at
+    q, k, v, o = (buf[:, a:a + n * D] for a, n in ((0, H), (256, Hk), (512, Hk), (1024, H)))
+    for i, t in enumerate((q, k, v)):
+        t.copy_(randn(i, T, t.shape[1]))
+    starts = [0, 69000, T]
+    off = i32(starts)
+    v[T - 3, 5] = float("inf")
+    o.fill_(11.0)
+    sp.attention_prompt(q, k, v, o, off, off, 2, T, T, H, Hk, D, ldq=ld, ldk=ld, ldv=ld, ldo=ld)
+    torch.cuda.synchronize()
+    for i in (68999, 69000, 69500, T - 200, T - 4):
+        a = max(s for s in starts if s <= i)
+        check(o[i:i + 1].reshape(1, H, D), *attend(q[i:i + 1].reshape(1, H, D), k[a:i + 1].reshape(-1, Hk, D), v[a:i + 1].reshape(-1, Hk, D), sp.F16, D ** -0.5, False))
+    assert not torch.isfinite(o[T - 3:].reshape(3, H, D)[..., 5]).any()
+    # few queries: CTAs of a cluster share the far keys
+    sp.attention_prompt(q[T - 40:], k, v, o[T - 40:], i32([0, 40]), i32([0, T]), 1, 40, T, H, Hk, D, ldq=ld, ldk=ld, ldv=ld, ldo=ld)
+    torch.cuda.synchronize()
+    for i in (T - 40, T - 4):
+        check(o[i:i + 1].reshape(1, H, D), *attend(q[i:i + 1].reshape(1, H, D), k[:i + 1].reshape(-1, Hk, D), v[:i + 1].reshape(-1, Hk, D), sp.F16, D ** -0.5, False))
+    del buf, q, k, v, o
+    torch.cuda.empty_cache()
